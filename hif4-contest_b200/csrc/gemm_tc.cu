@@ -33,12 +33,10 @@
 // Every mbarrier wait is bounded: on expiry the kernel records
 // HIF4X_TIMEOUT in a device status word and finishes without further
 // waits; hif4x_device_status() reports it.
-#include <cuda.h>
-
 #include <algorithm>
-#include <mutex>
 
 #include "common.cuh"
+#include "sm100.cuh"
 #include "tc_gemm.cuh"
 
 namespace hif4x {
@@ -70,7 +68,6 @@ struct Tile {
 };
 static_assert(Tile<128>::SMEM_BYTES <= 232448 && Tile<256>::SMEM_BYTES <= 232448, "shared memory per CTA");
 static_assert(Tile<256>::TMEM_COLS <= 512, "tensor memory columns");
-constexpr long long SPIN_LIMIT = 1ll << 22;
 // SMs a persistent GEMM leaves free: 16 of 148 took down_proj's calibration
 // (tensor-core Grams and Cholesky products beside one-CTA leaves and GPTQ
 // blocks on side streams) from 106.3 to 104 ms; 8, 24 and 36 did less well
@@ -78,36 +75,9 @@ constexpr int kTcFreeSms = 16;
 
 __device__ int g_status;   // sticky device status: 0 or HIF4X_TIMEOUT
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
 // bounded wait: false (and the device status set) if the phase never completes
 __device__ __forceinline__ bool mbar_wait_limit(uint64_t *bar, uint32_t parity, long long limit) {
-  for (long long i = 0; i < limit; i++)
-    if (mbar_try_wait(bar, parity)) return true;
-  atomicExch(&g_status, HIF4X_TIMEOUT);
-  return false;
+  return mbar_wait_limit(bar, parity, limit, &g_status);
 }
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
   return mbar_wait_limit(bar, parity, SPIN_LIMIT);
@@ -124,28 +94,6 @@ __global__ void wait_selftest_kernel(long long limit, int *done) {
   *done = ok ? 1 : 2;
 }
 
-__device__ __forceinline__ void tma_load_2d(const CUtensorMap *map, void *dst, uint64_t *bar, int x, int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-          smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
-      : "memory");
-}
-
-// UMMA shared-memory descriptor (sm100 version bits).  layout 2 = 128-byte
-// swizzle of 16-byte chunks (K-major tiles); layout 1 = 128-byte swizzle of
-// 32-byte chunks, the only MN-major layout for 32-bit (tf32) operands.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes,
-                                              uint32_t layout) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3fffu);
-  d |= (uint64_t)((lbo_bytes >> 4) & 0x3fffu) << 16;
-  d |= (uint64_t)((sbo_bytes >> 4) & 0x3fffu) << 32;
-  d |= (uint64_t)1 << 46;   // version (sm100)
-  d |= (uint64_t)layout << 61;
-  return d;
-}
-
 // Instruction descriptor: D fp32, A/B tf32, M = 128, N = BN_, majors.
 template <int BN_>
 __host__ __device__ constexpr uint32_t instr_desc(int a_mn_major, int b_mn_major) {
@@ -160,11 +108,6 @@ __device__ __forceinline__ void mma_tf32(uint32_t tmem_d, uint64_t adesc, uint64
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(tmem_d),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0));
-}
-
-__device__ __forceinline__ void mma_commit(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
 }
 
 // K-major operand descriptor of K-substep j (8 K-elements) of a 128 x 32
@@ -267,23 +210,12 @@ static int64_t tiles_of(int tm, int tn, int lower) {
   return n;
 }
 
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, const void *src, int x, int y) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
-                   reinterpret_cast<uint64_t>(map)),
-               "r"(smem_u32(src)), "r"(x), "r"(y)
-               : "memory");
-}
 __device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap *map, const void *src, int x, int y) {
   asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
                "r"(smem_u32(src)), "r"(x), "r"(y)
                : "memory");
 }
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-// the shared-memory source of all but the newest bulk group has been read
-__device__ __forceinline__ void bulk_wait_read_1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-
 template <int BN_>
 __global__ void __launch_bounds__(THREADS, 1) gemm_tc_kernel(const __grid_constant__ CUtensorMap mapA,
                                                              const __grid_constant__ CUtensorMap mapB,
@@ -675,23 +607,6 @@ __global__ void __launch_bounds__(256) split_tf32_vec_kernel(const float *__rest
 }
 
 // ------------------------------------------------------------------ host
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
-
 // 2-D fp32 tensor map over a split operand: `inner` (K) x `outer` (2R) floats,
 // row stride ld floats, 32 x box_rows boxes, 128-byte swizzle; K beyond
 // `inner` reads as zero.
@@ -722,12 +637,10 @@ static bool make_map_c(CUtensorMap *map, float *C, int64_t N, int64_t M, int64_t
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-constexpr int kMaxDevices = 64;
-
 // Per device: SM count, and the stream-ordered pool the split operands come
 // from set to keep its memory between calls (the split buffers are
 // allocated and freed around every product).
-static int device_sms(int dev) {
+int device_sms(int dev) {
   static int sms[kMaxDevices];
   static std::once_flag once[kMaxDevices];
   if (dev < 0 || dev >= kMaxDevices) return 0;
@@ -837,6 +750,18 @@ int gemm_split(const float *As, int a_products, const float *Bs, int b_products,
   else
     gemm_tc_kernel<128><<<(unsigned)grid, THREADS, Tile<128>::SMEM_BYTES, s>>>(ma, mb, mc, args);
   return cudaGetLastError() == cudaSuccess ? HIF4X_OK : HIF4X_ERR_LAUNCH;
+}
+
+// Device address of the sticky status word on device `dev` (the current one), looked up once; null on failure.
+int *status_word(int dev) {
+  static int *word[kMaxDevices];
+  static std::once_flag once[kMaxDevices];
+  if (dev < 0 || dev >= kMaxDevices) return nullptr;
+  std::call_once(once[dev], [dev] {
+    void *p = nullptr;
+    word[dev] = cudaGetSymbolAddress(&p, g_status) == cudaSuccess ? static_cast<int *>(p) : nullptr;
+  });
+  return word[dev];
 }
 
 }  // namespace tc
