@@ -1,0 +1,82 @@
+// hif4_bits.cuh -- packed HiF4 -> bf16 in registers, for the kernels that
+// multiply by packed values.
+//
+// An element is +-(m/4) sf 2^(lv2 + lv3) with m in 0..7 and sf = (4 + M)/4
+// 2^E: m (4 + M) <= 49 takes six significant bits, so every HiF4 value is a
+// bf16 number and a product with it loses nothing before the fp32 sum.
+//
+// Decode: a word of eight sign-magnitude nibbles becomes eight offset
+// nibbles 8 + v (v = +-m; five integer operations for the word), two of which
+// are dropped into the mantissas of a bf16 pair 128 + (8 + v), and one
+// bf16x2 FMA takes the offset away and applies the scale:
+//   (136 + v) S - 136 S = v S,   S = sf/4 2^(lv2 + lv3),
+// exact: 136 S has at most seven significant bits, v S at most six.
+// About 3.5 instructions per element with the scales, against 5 and more for
+// extracting sign and magnitude one by one.
+#pragma once
+#include "common.cuh"
+
+namespace hif4x {
+
+// nibbles sign << 3 | m -> 8 + m or 8 - m (no carry leaves a nibble)
+__device__ __forceinline__ uint32_t hif4_offset(uint32_t w) {
+  const uint32_t neg7 = ((w >> 3) & 0x11111111u) * 7u;   // 7 in each negative nibble
+  return ((w & 0x77777777u) ^ neg7) + (0x88888888u - neg7);
+}
+
+__device__ __forceinline__ uint32_t bf16x2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t bf16x2_mul(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+constexpr uint32_t kNeg136 = 0xc308c308u;   // bf16 pair -136
+
+// bf16 bits of sf/4 in both halves: the E6M2 byte (E + 48) << 2 | M is the
+// top of a bf16 significand, so its exponent is rebased by one addition
+__device__ __forceinline__ uint32_t hif4_sf2(uint32_t meta) { return (meta & 0xffu) * 0x00200020u + 0x26802680u; }
+
+// The scales of sub-block i (8 elements): quad 0 and quad 1, each in both halves.
+__device__ __forceinline__ void hif4_scales(uint32_t meta, uint32_t sf2, int i, uint32_t &s0, uint32_t &s1) {
+  const uint32_t b = ((meta >> (8 + i)) & 1u) * 0x00800080u + sf2;
+  s0 = ((meta >> (16 + 2 * i)) & 1u) * 0x00800080u + b;
+  s1 = ((meta >> (17 + 2 * i)) & 1u) * 0x00800080u + b;
+}
+
+// Word of sub-block i -> four bf16 pairs in element order (0,1) (2,3) (4,5) (6,7).
+__device__ __forceinline__ void hif4_decode8(uint32_t w, uint32_t meta, uint32_t sf2, int i, uint32_t (&o)[4]) {
+  uint32_t s0, s1;
+  hif4_scales(meta, sf2, i, s0, s1);
+  const uint32_t z0 = bf16x2_mul(s0, kNeg136), z1 = bf16x2_mul(s1, kNeg136);
+  const uint32_t lo = hif4_offset(w), hi = lo >> 4;
+  // element 2p is nibble 2p (byte p of lo), element 2p + 1 the low nibble of byte p of hi
+  o[0] = bf16x2_fma((__byte_perm(lo, hi, 0x0400) & 0x000f000fu) | 0x43004300u, s0, z0);
+  o[1] = bf16x2_fma((__byte_perm(lo, hi, 0x0501) & 0x000f000fu) | 0x43004300u, s0, z0);
+  o[2] = bf16x2_fma((__byte_perm(lo, hi, 0x0602) & 0x000f000fu) | 0x43004300u, s1, z1);
+  o[3] = bf16x2_fma((__byte_perm(lo, hi, 0x0703) & 0x000f000fu) | 0x43004300u, s1, z1);
+}
+
+// Where new row `token` of a batch belongs: its sequence (cu_new[s] <= token
+// < cu_new[s + 1]) and its position kv_len[s] - (cu_new[s + 1] - token).
+// Eight lanes of a warp (aligned, `mask` of them) search together, eight
+// pivots a step.  seq = B: behind the last sequence.
+__device__ __forceinline__ int find_sequence(const int *cu_new, int B, int64_t token, int sub, unsigned mask) {
+  int lo = 0, hi = B;   // the answer: how many of cu_new[1..B] are <= token
+  while (lo < hi) {
+    const int at = min(hi, lo + 1 + (int)(((int64_t)sub * (hi - lo)) >> 3));
+    const unsigned le = __ballot_sync(mask, (int64_t)cu_new[at] <= token) & mask;
+    const int n = __popc(le);   // cu_new does not fall, so these are the first n pivots
+    const int r = hi - lo;
+    const int last = n == 0 ? lo : min(hi, lo + 1 + (int)(((int64_t)(n - 1) * r) >> 3));
+    const int next = n == 8 ? hi : min(hi, lo + 1 + (int)(((int64_t)n * r) >> 3)) - 1;
+    lo = last;
+    hi = max(last, next);
+  }
+  return lo;
+}
+
+}  // namespace hif4x

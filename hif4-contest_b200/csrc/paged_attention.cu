@@ -1,0 +1,510 @@
+// paged_attention.cu -- softmax attention of new tokens over the paged HiF4
+// cache: o = sum_t softmax_t(scale q.k_t) v_t over the visible keys t.
+//
+// Query row j of a sequence of length L with n new rows stands at position
+// p = L - n + j and sees the keys t <= p with t > p - window or t < sinks.
+//
+// attend_rows_kernel (few rows per key head: single tokens, drafts) is bound
+// by the cache's bytes and by the instructions that turn them into bf16, so
+// it reads each packed byte once, straight into the registers of the thread
+// that multiplies it, and keeps no tile in shared memory:
+//   S^T = K Q^T, O^T = V^T P^T with mma.m16n8k16: 16 keys (then 16 of the
+//   head's dims) are the M side and 8 query rows the N side, so a group of
+//   up to 8 query heads wastes no half of the instruction.
+//   K: the contraction runs over the dims, whose order is free as long as Q
+//   has the same one: thread c of a key's four holds dims c dh/4 .. +dh/4,
+//   one 16-byte load, and pairs nibbles j and j + 4 of a word (a shift and a
+//   mask, and the pair's scales are the two quads' of one sub-block).
+//   V: the contraction runs over keys, so a pair is one dim of two keys: two
+//   byte permutes make two words of code pairs out of both keys' words.
+// The softmax reference of a row moves only when a score passes it by 2^8:
+// weights are then at most 256, and any reference gives the same quotient,
+// so the common tile needs one vote and no shuffle and no rescaling.
+// A warp takes every fourth 16-key tile of its CTA's share; the warps' sums
+// meet in shared memory, the shares of one (sequence, key head) in a second
+// kernel that adds them in order (the result does not depend on timing).
+#include <algorithm>
+
+#include "common.cuh"
+#include "hif4_bits.cuh"
+#include "kvcache.cuh"
+#include "sm100.cuh"
+
+namespace hif4x {
+
+struct AttendArgs {
+  CacheArgs c;
+  const __nv_bfloat16 *q;
+  int64_t q_row, q_head;      // strides in elements, multiples of 8
+  __nv_bfloat16 *out;
+  int64_t o_row, o_head;
+  int group;                  // query heads per key head
+  float scale;                // times log2(e)
+  int window, sinks;          // window 0: all keys
+  int splits;
+  float *part;                // (splits, rows, q heads, dh) sums, then (splits, rows, q heads) (reference, weight)
+  float2 *part_ml;
+};
+
+constexpr float kLazy = 8.0f;    // log2 a row's scores may pass its reference by
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The 16-key tiles a run of positions [p_lo, p_hi] of one sequence can see:
+// the sinks' tiles, then those from the window's first key to p_hi.
+struct KeyTiles {
+  int n_sink, n, first;   // tiles; the first window tile
+  __device__ __forceinline__ KeyTiles(int p_lo, int p_hi, int window, int sinks, int tile) {
+    first = 0;
+    n_sink = 0;
+    if (p_hi < 0) {
+      n = 0;
+      return;
+    }
+    if (window > 0 && p_lo - window + 1 > 0) {
+      first = (p_lo - window + 1) / tile;
+      n_sink = min(first, (sinks + tile - 1) / tile);
+    }
+    n = n_sink + p_hi / tile - first + 1;
+  }
+  __device__ __forceinline__ int key0(int i, int tile) const { return (i < n_sink ? i : i - n_sink + first) * tile; }
+};
+
+// One 16-key tile's packed words in registers.
+template <int DH>
+struct TileRegs {
+  uint32_t k[2][DH / 32], km[2], v[4][DH / 64], vm[4];
+  __device__ __forceinline__ void load(const CacheArgs &c, int64_t row, int lane) {
+    const int n = lane >> 2, q = lane & 3;
+    constexpr int NB = DH / 64;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int64_t r = row + n + 8 * u;
+      if (DH == 128) {
+        const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(c.codes[0] + r * (DH / 2)) + q);
+        k[u][0] = w.x;
+        k[u][1] = w.y;
+        k[u][DH / 32 - 2] = w.z;
+        k[u][DH / 32 - 1] = w.w;
+      } else {
+        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(c.codes[0] + r * (DH / 2)) + q);
+        k[u][0] = w.x;
+        k[u][1] = w.y;
+      }
+      km[u] = __ldcs(c.meta[0] + r * NB + (DH == 128 ? q >> 1 : 0));
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int64_t r = row + 2 * q + (u & 1) + 8 * (u >> 1);
+      if (DH == 128) {
+        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(c.codes[1] + r * (DH / 2)) + n);
+        v[u][0] = w.x;
+        v[u][DH / 64 - 1] = w.y;
+      } else {
+        v[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(c.codes[1] + r * (DH / 2)) + n);
+      }
+      vm[u] = __ldcs(c.meta[1] + r * NB + (DH == 128 ? n >> 2 : 0));
+    }
+  }
+};
+
+// DH: head dim; NT: query rows / 8 of a row tile.
+template <int DH, int NT>
+__global__ void __launch_bounds__(128) attend_rows_kernel(const AttendArgs a) {
+  constexpr int WARPS = 4, KW = DH / 32, ROWS = 8 * NT;
+  __shared__ float so[WARPS][ROWS][DH + 4];
+  __shared__ float2 sml[WARPS][ROWS];
+  const CacheArgs &c = a.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n8 = lane >> 2, q4 = lane & 3;
+  const int s = blockIdx.x, kh = blockIdx.y, split = blockIdx.z;
+  const int cu0 = c.cu_new[s], n_new = c.cu_new[s + 1] - cu0;
+  if (n_new <= 0) return;
+  const int64_t room = (int64_t)c.most << c.page_shift;
+  const int old = c.kv_len[s] - n_new;   // position of the first new row
+  const int *pages = c.pages + s * c.ld_pages;
+  const int64_t rows = (int64_t)n_new * a.group;
+
+  for (int64_t r0 = 0; r0 < rows; r0 += ROWS) {
+    const int64_t r1 = min(rows, r0 + ROWS);
+    const int p_lo = old + (int)(r0 / a.group);
+    const int p_top = old + (int)((r1 - 1) / a.group);
+    int p_hi = p_top;
+    if (p_hi >= room) {   // the table has no page for its last keys
+      if (threadIdx.x == 0) atomicExch(c.status, HIF4X_BAD_PAGE);
+      p_hi = (int)(room - 1);
+    }
+    // this thread's Q fragments: row r0 + 8 nt + n8, dims q4 dh/4 .. in pairs (j, j + 4)
+    uint32_t qf[NT][KW * 4];
+    int pos[NT][2];   // positions of the rows 8 nt + 2 q4 + {0, 1} whose scores this thread has
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const int64_t r = r0 + 8 * nt + n8;
+      const int64_t token = (int64_t)cu0 + r / a.group;
+      const bool ok = r < r1 && token >= 0 && token < c.rows;
+      const uint4 *src = reinterpret_cast<const uint4 *>(
+          a.q + (ok ? token * a.q_row + (kh * a.group + (int)(r % a.group)) * a.q_head + q4 * (DH / 4) : 0));
+#pragma unroll
+      for (int w = 0; w < KW; w++) {
+        const uint4 x = ok ? __ldg(src + w) : make_uint4(0, 0, 0, 0);   // dims 8w .. 8w + 7
+        qf[nt][4 * w + 0] = __byte_perm(x.x, x.z, 0x5410);
+        qf[nt][4 * w + 1] = __byte_perm(x.x, x.z, 0x7632);
+        qf[nt][4 * w + 2] = __byte_perm(x.y, x.w, 0x5410);
+        qf[nt][4 * w + 3] = __byte_perm(x.y, x.w, 0x7632);
+      }
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        const int64_t rr = r0 + 8 * nt + 2 * q4 + b;
+        pos[nt][b] = rr < r1 ? old + (int)(rr / a.group) : -1;
+      }
+    }
+    float o[DH / 16][NT][4], ref[NT][2], sum[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        ref[nt][b] = -INFINITY;
+        sum[nt][b] = 0.0f;
+      }
+#pragma unroll
+      for (int mt = 0; mt < DH / 16; mt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[mt][nt][e] = 0.0f;
+    }
+
+    const KeyTiles tiles(min(max(p_lo, 0), p_hi), p_hi, a.window, a.sinks, 16);
+    const int per = (tiles.n + a.splits - 1) / a.splits;
+    const int t1 = min(tiles.n, (split + 1) * per);
+    int t = split * per + warp;
+    // the page of a tile two ahead, the words of the next one
+    auto page_of = [&](int i) -> int {
+      if (i >= t1) return -1;
+      const int pg = __ldg(pages + (tiles.key0(i, 16) >> c.page_shift));
+      if (pg >= 0 && pg < c.num_pages) return pg;
+      if (lane == 0) atomicExch(c.status, HIF4X_BAD_PAGE);
+      return -1;
+    };
+    auto row_of = [&](int i, int pg) -> int64_t {
+      return ((int64_t)pg * c.heads + kh) * c.page_size + (tiles.key0(i, 16) & (c.page_size - 1));
+    };
+    TileRegs<DH> cur, next;
+    int pg = page_of(t), pg_next = page_of(t + WARPS);
+    if (pg >= 0) cur.load(c, row_of(t, pg), lane);
+    for (; t < t1; t += WARPS) {
+      const int pg_next2 = page_of(t + 2 * WARPS);
+      if (pg_next >= 0) next.load(c, row_of(t + WARPS, pg_next), lane);
+      if (pg >= 0) {
+        const int key0 = tiles.key0(t, 16);
+        // ---- scores: S^T (16 keys x 8 NT rows)
+        float sc[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) sc[nt][e] = 0.0f;
+        const uint32_t sf0 = hif4_sf2(cur.km[0]), sf1 = hif4_sf2(cur.km[1]);
+#pragma unroll
+        for (int w = 0; w < KW; w++) {
+          const int i = (DH == 128 ? (q4 & 1) * 4 : q4 * 2) + w;   // sub-block of the group
+          uint32_t a0, a1, b0, b1;
+          hif4_scales(cur.km[0], sf0, i, a0, a1);
+          hif4_scales(cur.km[1], sf1, i, b0, b1);
+          const uint32_t s0 = __byte_perm(a0, a1, 0x5410), s1 = __byte_perm(b0, b1, 0x5410);
+          const uint32_t z0 = bf16x2_mul(s0, kNeg136), z1 = bf16x2_mul(s1, kNeg136);
+          const uint32_t x0 = hif4_offset(cur.k[0][w]), x1 = hif4_offset(cur.k[1][w]);
+          uint32_t f[4][2];
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            f[j][0] = bf16x2_fma(((x0 >> (4 * j)) & 0x000f000fu) | 0x43004300u, s0, z0);
+            f[j][1] = bf16x2_fma(((x1 >> (4 * j)) & 0x000f000fu) | 0x43004300u, s1, z1);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const uint32_t fa[4] = {f[2 * h][0], f[2 * h][1], f[2 * h + 1][0], f[2 * h + 1][1]};
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) mma_bf16(sc[nt], fa, qf[nt][4 * w + 2 * h], qf[nt][4 * w + 2 * h + 1]);
+          }
+        }
+        // ---- mask; scores to log2 units.  sc[e]: key key0 + n8 + 8 (e >> 1), row 8 nt + 2 q4 + (e & 1)
+        const bool all = key0 + 15 <= p_lo && (a.window == 0 || key0 > p_top - a.window || key0 + 15 < a.sinks);
+        bool over = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            sc[nt][e] *= a.scale;
+            if (!all) {
+              const int key = key0 + n8 + 8 * (e >> 1), p = pos[nt][e & 1];
+              if (!(key <= p && (a.window == 0 || key > p - a.window || key < a.sinks))) sc[nt][e] = -INFINITY;
+            }
+            over |= sc[nt][e] > ref[nt][e & 1] + kLazy;
+          }
+        if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+              float m = fmaxf(ref[nt][b], fmaxf(sc[nt][b], sc[nt][2 + b]));
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+              const float f = ref[nt][b] == -INFINITY ? 0.0f : ex2(ref[nt][b] - m);
+              ref[nt][b] = m;
+              sum[nt][b] *= f;
+#pragma unroll
+              for (int mt = 0; mt < DH / 16; mt++) {
+                o[mt][nt][b] *= f;
+                o[mt][nt][2 + b] *= f;
+              }
+            }
+        }
+        // ---- weights, transposed for the second product
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float m = ref[nt][e & 1];
+            p[e] = ex2(sc[nt][e] - (m == -INFINITY ? 0.0f : m));
+            sum[nt][e & 1] += p[e];
+          }
+          pb[nt][0] = transpose8x8(pack_bf16(p[0], p[1]));
+          pb[nt][1] = transpose8x8(pack_bf16(p[2], p[3]));
+        }
+        // ---- O^T (dh x 8 NT) += V^T P^T
+        uint32_t vsf[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) vsf[u] = hif4_sf2(cur.vm[u]);
+#pragma unroll
+        for (int w = 0; w < DH / 64; w++) {
+          const int i = DH == 128 ? (n8 & 3) * 2 + w : n8;   // sub-block of the group
+          uint32_t sk[4][2], x[4];
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            hif4_scales(cur.vm[u], vsf[u], i, sk[u][0], sk[u][1]);
+            x[u] = hif4_offset(cur.v[u][w]);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; h++) {   // quad: dims 4h .. 4h + 3 of the word
+            const uint32_t s01 = __byte_perm(sk[0][h], sk[1][h], 0x5410), s23 = __byte_perm(sk[2][h], sk[3][h], 0x5410);
+            const uint32_t z01 = bf16x2_mul(s01, kNeg136), z23 = bf16x2_mul(s23, kNeg136);
+            const uint32_t y01 = __byte_perm(x[0], x[1], h ? 0x7632 : 0x5410);
+            const uint32_t y23 = __byte_perm(x[2], x[3], h ? 0x7632 : 0x5410);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+              const uint32_t fa[4] = {
+                  bf16x2_fma(((y01 >> (8 * j)) & 0x000f000fu) | 0x43004300u, s01, z01),
+                  bf16x2_fma(((y01 >> (8 * j + 4)) & 0x000f000fu) | 0x43004300u, s01, z01),
+                  bf16x2_fma(((y23 >> (8 * j)) & 0x000f000fu) | 0x43004300u, s23, z23),
+                  bf16x2_fma(((y23 >> (8 * j + 4)) & 0x000f000fu) | 0x43004300u, s23, z23)};
+#pragma unroll
+              for (int nt = 0; nt < NT; nt++) mma_bf16(o[w * 4 + h * 2 + j][nt], fa, pb[nt][0], pb[nt][1]);
+            }
+          }
+        }
+      }
+      cur = next;
+      pg = pg_next;
+      pg_next = pg_next2;
+    }
+
+    // ---- the four warps' sums: row 8 nt + 2 q4 + b, dims n8 dh/8 + 2 mt + {0, 1}
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        float l = sum[nt][b];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+        const int r = 8 * nt + 2 * q4 + b;
+        if (n8 == 0) sml[warp][r] = make_float2(ref[nt][b], l);
+#pragma unroll
+        for (int mt = 0; mt < DH / 16; mt++)
+          *reinterpret_cast<float2 *>(&so[warp][r][n8 * (DH / 8) + 2 * mt]) = make_float2(o[mt][nt][b], o[mt][nt][2 + b]);
+      }
+    __syncthreads();
+    for (int e = threadIdx.x; e < ROWS * (DH / 4); e += 128) {
+      const int r = e / (DH / 4), d = (e % (DH / 4)) * 4;
+      const int64_t rr = r0 + r, token = (int64_t)cu0 + rr / a.group;
+      if (rr >= r1 || token < 0 || token >= c.rows) continue;
+      float m = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WARPS; w++) m = fmaxf(m, sml[w][r].x);
+      float l = 0.0f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < WARPS; w++) {
+        const float2 ml = sml[w][r];
+        const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m);
+        l += f * ml.y;
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] += f * so[w][r][d + k];
+      }
+      const int head = kh * a.group + (int)(rr % a.group);
+      if (a.splits == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        *reinterpret_cast<uint2 *>(a.out + token * a.o_row + head * a.o_head + d) =
+            make_uint2(pack_bf16(v[0] * inv, v[1] * inv), pack_bf16(v[2] * inv, v[3] * inv));
+      } else {
+        const int64_t at = ((int64_t)split * c.rows + token) * (c.heads * a.group) + head;
+        *reinterpret_cast<float4 *>(a.part + at * DH + d) = make_float4(v[0], v[1], v[2], v[3]);
+        if (d == 0) a.part_ml[at] = make_float2(m, l);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// The shares of a (row, query head), added in their order: a warp each.
+template <int DH>
+__global__ void __launch_bounds__(128) attend_join_kernel(const AttendArgs a) {
+  const CacheArgs &c = a.c;
+  const int heads = c.heads * a.group, lane = threadIdx.x & 31;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5), all = c.rows * heads;
+  if (at >= all) return;
+  const int64_t token = at / heads;
+  const int head = (int)(at - token * heads);
+  if (token < c.cu_new[0] || token >= c.cu_new[c.B]) return;   // rows of no sequence stay as they are
+  constexpr int V = DH / 32;
+  float m = -INFINITY;
+  for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, a.part_ml[s * all + at].x);
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+  float l = 0.0f, v[V];
+#pragma unroll
+  for (int k = 0; k < V; k++) v[k] = 0.0f;
+  for (int s = 0; s < a.splits; s++) {
+    const float2 ml = a.part_ml[s * all + at];
+    if (ml.x == -INFINITY) continue;   // nothing visible in this share
+    const float f = ex2(ml.x - m);
+    l += f * ml.y;
+    const float *src = a.part + (s * all + at) * DH + lane * V;
+#pragma unroll
+    for (int k = 0; k < V; k++) v[k] += f * src[k];
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint32_t *dst = reinterpret_cast<uint32_t *>(a.out + token * a.o_row + head * a.o_head + lane * V);
+#pragma unroll
+  for (int k = 0; k < V / 2; k++) dst[k] = pack_bf16(v[2 * k] * inv, v[2 * k + 1] * inv);
+}
+
+// Shares of the keys of one (sequence, key head): enough CTAs for four on
+// every SM, none with fewer than two tiles for each of its warps, and no more
+// than 2^26 partial sums (256 MB) in all.
+static int attend_splits(int sms, int64_t lanes, int64_t keys, int64_t outputs) {
+  const int64_t want = (4 * (int64_t)sms + lanes - 1) / lanes, most = std::max<int64_t>(1, keys / (16 * 4 * 2));
+  const int64_t room = (int64_t(1) << 26) / std::max<int64_t>(1, outputs);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, room, 256}));
+}
+
+// How a call is carried out: from its sizes alone.
+struct AttendPlan {
+  int splits;
+  int64_t part_floats, work_bytes;
+};
+
+static int attend_plan(const hif4x_kv_cache *kv, const hif4x_kv_batch *b, int q_heads, int64_t rows, int window,
+                       int sinks, int max_new, AttendPlan *p) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return HIF4X_ERR_LAUNCH;
+  const int sms = tc::device_sms(dev);
+  if (sms <= 0) return HIF4X_ERR_LAUNCH;
+  int64_t keys = (int64_t)b->max_pages * kv->page_size;
+  if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + max_new + sinks + 32);
+  p->splits = attend_splits(sms, (int64_t)b->sequences * kv->kv_heads, keys, rows * q_heads * kv->head_dim);
+  p->part_floats = p->splits > 1 ? (int64_t)p->splits * rows * q_heads * kv->head_dim : 0;
+  p->work_bytes = p->splits > 1 ? p->part_floats * 4 + (int64_t)p->splits * rows * q_heads * 8 : 0;
+  return HIF4X_OK;
+}
+
+static int attend_check(const hif4x_kv_cache *kv, const hif4x_kv_batch *b, int q_heads, int64_t rows, int window,
+                        int sinks, int max_new, CacheArgs *c) {
+  const int st = cache_args(kv, b, rows, c);
+  if (st != HIF4X_OK) return st;
+  if (q_heads < kv->kv_heads || q_heads % kv->kv_heads || window < 0 || sinks < 0 || max_new < 1 ||
+      window > (1 << 30) || sinks > (1 << 30) || rows * q_heads > INT32_MAX)
+    return HIF4X_ERR_ARG;
+  return HIF4X_OK;
+}
+
+}  // namespace hif4x
+
+using namespace hif4x;
+
+extern "C" int hif4x_paged_attention_work(const hif4x_kv_cache *kv, const hif4x_kv_batch *batch, int q_heads,
+                                          int64_t rows, int window, int sinks, int max_new, int64_t *bytes) {
+  if (!bytes) return HIF4X_ERR_ARG;
+  CacheArgs c{};
+  const int st = attend_check(kv, batch, q_heads, rows, window, sinks, max_new, &c);
+  if (st != HIF4X_OK) return st;
+  AttendPlan p{};
+  const int st2 = attend_plan(kv, batch, q_heads, rows, window, sinks, max_new, &p);
+  *bytes = p.work_bytes;
+  return st2;
+}
+
+extern "C" int hif4x_paged_attention(const hif4x_kv_cache *kv, const hif4x_kv_batch *batch, const void *q,
+                                     int64_t q_ld_row, int64_t q_ld_head, int q_heads, int64_t rows, float scale,
+                                     int window, int sinks, int max_new, void *out, int64_t o_ld_row,
+                                     int64_t o_ld_head, void *work, int64_t work_bytes, void *stream) {
+  AttendArgs a{};
+  int st = attend_check(kv, batch, q_heads, rows, window, sinks, max_new, &a.c);
+  if (st != HIF4X_OK) return st;
+  if (rows == 0) return HIF4X_OK;
+  if (!q || !out || q == out) return HIF4X_ERR_ARG;
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) || q_ld_row % 8 || q_ld_head % 8 ||
+      o_ld_row % 8 || o_ld_head % 8)
+    return HIF4X_ERR_ARG;
+  AttendPlan p{};
+  st = attend_plan(kv, batch, q_heads, rows, window, sinks, max_new, &p);
+  if (st != HIF4X_OK) return st;
+  if (p.work_bytes > 0 && (!work || work_bytes < p.work_bytes || (reinterpret_cast<uintptr_t>(work) & 15u)))
+    return HIF4X_ERR_ARG;
+  a.q = static_cast<const __nv_bfloat16 *>(q);
+  a.q_row = q_ld_row;
+  a.q_head = q_ld_head;
+  a.out = static_cast<__nv_bfloat16 *>(out);
+  a.o_row = o_ld_row;
+  a.o_head = o_ld_head;
+  a.group = q_heads / kv->kv_heads;
+  a.scale = scale * 1.4426950408889634f;
+  a.window = window;
+  a.sinks = sinks;
+  a.splits = p.splits;
+  a.part = static_cast<float *>(work);
+  a.part_ml = reinterpret_cast<float2 *>(static_cast<float *>(work) + p.part_floats);
+  cudaStream_t s = (cudaStream_t)stream;
+  const dim3 grid((unsigned)batch->sequences, (unsigned)kv->kv_heads, (unsigned)p.splits);
+  const bool two = (int64_t)max_new * a.group > 8;
+  if (kv->head_dim == 128) {
+    if (two) attend_rows_kernel<128, 2><<<grid, 128, 0, s>>>(a);
+    else attend_rows_kernel<128, 1><<<grid, 128, 0, s>>>(a);
+  } else {
+    if (two) attend_rows_kernel<64, 2><<<grid, 128, 0, s>>>(a);
+    else attend_rows_kernel<64, 1><<<grid, 128, 0, s>>>(a);
+  }
+  HIF4X_CHECK_LAUNCH();
+  if (p.splits > 1) {
+    const unsigned blocks = (unsigned)((rows * q_heads + 3) / 4);
+    if (kv->head_dim == 128) attend_join_kernel<128><<<blocks, 128, 0, s>>>(a);
+    else attend_join_kernel<64><<<blocks, 128, 0, s>>>(a);
+    HIF4X_CHECK_LAUNCH();
+  }
+  return HIF4X_OK;
+}

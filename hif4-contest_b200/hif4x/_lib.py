@@ -14,7 +14,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 SO_PATH = os.path.join(_HERE, "libhif4x.so")
 
-OK, NOT_PD, TIMEOUT = 0, 1, 2
+OK, NOT_PD, TIMEOUT, BAD_PAGE = 0, 1, 2, 3
 ERR_ARG, ERR_LAUNCH, ERR_UNSUPPORTED, ERR_SCRATCH, ERR_NOMEM = -1, -2, -3, -4, -5
 DT_F32, DT_BF16, DT_F64 = 0, 1, 2
 SRC_NVFP4_PACKED, SRC_NVFP4_PAIR, SRC_VALUES = 0, 1, 2
@@ -22,6 +22,7 @@ SMOOTH_NONE, SMOOTH_MUL, SMOOTH_DIV = 0, 1, 2
 ENC_NONE, ENC_SEARCH, ENC_FAST, ENC_ALG1 = 0, 1, 2, 3
 
 _STATUS = {OK: "ok", NOT_PD: "not positive definite", TIMEOUT: "device wait timed out",
+           BAD_PAGE: "a page table named no page of the cache",
            ERR_ARG: "bad argument", ERR_LAUNCH: "CUDA launch error", ERR_UNSUPPORTED: "unsupported",
            ERR_SCRATCH: "size above the static scratch maximum",
            ERR_NOMEM: "out of device memory for a workspace"}
@@ -45,6 +46,16 @@ class ConvertDesc(ctypes.Structure):
                 ("rot_signs", vp), ("encode_mode", i32), ("out_x", vp), ("sf", vp), ("lv2", vp), ("lv3", vp),
                 ("sign", vp), ("mant", vp), ("meta", vp), ("codes", vp), ("deq", vp), ("deq_dtype", i32),
                 ("unit", vp)]
+
+
+class KVCacheDesc(ctypes.Structure):
+    _fields_ = [("k_codes", vp), ("k_meta", vp), ("v_codes", vp), ("v_meta", vp), ("num_pages", i64),
+                ("page_size", i32), ("kv_heads", i32), ("head_dim", i32)]
+
+
+class KVBatchDesc(ctypes.Structure):
+    _fields_ = [("cu_new", vp), ("kv_len", vp), ("pages", vp), ("sequences", i32), ("max_pages", i32),
+                ("ld_pages", i64)]
 
 
 # name -> argtypes (restype is int for every entry point)
@@ -102,6 +113,14 @@ SIGNATURES: dict[str, list] = {
     "hif4x_e2m1_pack": [vp, i32, i64, vp, vp, vp],
     "hif4x_e2m1_unpack": [vp, i64, vp, i32, vp],
     "hif4x_hif4_rows": [vp, vp, i64, i64, vp, vp],
+    "hif4x_linear_packed": [vp, i64, vp, vp, i64, i64, i64, vp, i32, i32, vp, i64, vp, i64, vp],
+    "hif4x_kv_append": [ctypes.POINTER(KVCacheDesc), ctypes.POINTER(KVBatchDesc), vp, i64, i64, vp, i64, i64, i32,
+                        i64, vp],
+    "hif4x_kv_read": [ctypes.POINTER(KVCacheDesc), ctypes.POINTER(KVBatchDesc), i64, vp, vp, i32, vp],
+    "hif4x_paged_attention_work": [ctypes.POINTER(KVCacheDesc), ctypes.POINTER(KVBatchDesc), i32, i64, i32, i32, i32,
+                                   ctypes.POINTER(i64)],
+    "hif4x_paged_attention": [ctypes.POINTER(KVCacheDesc), ctypes.POINTER(KVBatchDesc), vp, i64, i64, i32, i64, f32,
+                              i32, i32, i32, vp, i64, i64, vp, i64, vp],
 }
 
 _LIB = None

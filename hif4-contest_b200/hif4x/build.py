@@ -1,6 +1,6 @@
 """Build libhif4x.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a.
 
-Each csrc/*.cu is compiled separately (codec.cu with -fmad=false as a
+Each csrc/*.cu is compiled separately (codec.cu, kvcache.cu with -fmad=false as a
 safety net: its arithmetic is written with explicit round-to-nearest
 intrinsics and must never be contracted) and linked into
 hif4x/libhif4x.so next to this file.  Rebuilds only when a source or header
@@ -23,7 +23,7 @@ SO = os.path.join(PKG, "libhif4x.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
           "-I", INCLUDE, "-I", CSRC]
-PER_FILE = {"codec.cu": ["-fmad=false"]}
+PER_FILE = {"codec.cu": ["-fmad=false"], "kvcache.cu": ["-fmad=false"]}
 
 
 def _nvcc() -> str:

@@ -39,6 +39,7 @@ extern "C" {
 #define HIF4X_OK 0
 #define HIF4X_NOT_PD 1            /* Cholesky met a non-positive pivot        */
 #define HIF4X_TIMEOUT 2           /* a bounded device wait gave up            */
+#define HIF4X_BAD_PAGE 3          /* a page table named no page of the cache  */
 #define HIF4X_ERR_ARG (-1)        /* bad pointer / size / alignment           */
 #define HIF4X_ERR_LAUNCH (-2)     /* CUDA launch or runtime error             */
 #define HIF4X_ERR_UNSUPPORTED (-3)
@@ -202,7 +203,10 @@ int hif4x_gemm_tc(int ta, int tb, int64_t M, int64_t N, int64_t K, float alpha, 
                   const float *B, int64_t ldb, float beta, float *C, int64_t ldc, void *stream);
 
 /* Synchronises the stream; returns (and clears) the sticky device status:
- * HIF4X_TIMEOUT if a bounded device-side wait expired since the last call.
+ * HIF4X_TIMEOUT if a bounded device-side wait expired since the last call,
+ * HIF4X_BAD_PAGE if a kernel of the key/value cache met a position whose page
+ * table entry names no page (the row is not written, the keys count as
+ * hidden); the later of the two where both happened.
  * One status word per device (not per stream): a read clears it for every
  * stream of that device. */
 int hif4x_device_status(void *stream);
@@ -369,6 +373,82 @@ int hif4x_transpose_batched(const float *in, int64_t R, int64_t Cc, int64_t batc
                             float *out, int64_t old, int64_t obs, void *stream);
 /* fp32 round-to-nearest of f64 (G.float(), solution.py:1327). */
 int hif4x_f64_to_f32(const double *in, int64_t n, float *out, void *stream);
+
+/* ---- serving: products with packed weights (csrc/linear.cu) ------------ */
+
+#define HIF4X_ACT_NONE 0
+#define HIF4X_ACT_RELU 1
+#define HIF4X_ACT_GELU 2          /* x Phi(x), by erf                         */
+#define HIF4X_ACT_GELU_TANH 3     /* its tanh form                            */
+#define HIF4X_ACT_SILU 4          /* x / (1 + exp(-x))                        */
+
+/* y = act(x W^T + bias) + residual with W in packed HiF4 (no counterpart in
+ * the reference, which multiplies decoded values: solution.py:860-1025).
+ * x: T x C bf16, row stride ldx (a multiple of 8), 16-byte aligned; W: meta
+ * (N, C/64), codes (N, C/2), 16-byte aligned; bias: N values of bias_dtype
+ * (HIF4X_DT_F32 or HIF4X_DT_BF16) or NULL; residual: T x N bf16, row stride
+ * ldr, or NULL; y: T x N bf16, row stride ldy, may be the residual itself.
+ * C % 64 == 0.  W's values are exact in bf16, products are summed in fp32 on
+ * the tensor cores (tcgen05), the sum is rounded once. */
+int hif4x_linear_packed(const void *x, int64_t ldx, const uint32_t *meta, const uint8_t *codes, int64_t T, int64_t N,
+                        int64_t C, const void *bias, int bias_dtype, int act, const void *residual, int64_t ldr,
+                        void *y, int64_t ldy, void *stream);
+
+/* ---- serving: paged HiF4 key/value cache (csrc/kvcache.cu) -------------- */
+
+/* A cache: for K and V the packed unit of every head's row, a head's tokens of
+ * one page together: codes (num_pages, kv_heads, page_size, head_dim/2) bytes,
+ * meta (num_pages, kv_heads, page_size, head_dim/64) words, 16-byte aligned.
+ * head_dim 64 or 128; page_size a power of two, 16 to 256. */
+typedef struct hif4x_kv_cache {
+  void *k_codes, *k_meta, *v_codes, *v_meta;
+  int64_t num_pages;
+  int page_size, kv_heads, head_dim;
+} hif4x_kv_cache;
+
+/* A batch of sequences with new rows, all on the device: sequence s has the
+ * rows cu_new[s] .. cu_new[s+1] - 1 of the batch's tensors (cu_new does not
+ * fall; rows from cu_new[sequences] on belong to no sequence), kv_len[s]
+ * tokens with the new ones, and pages[s * ld_pages + i] holds its tokens
+ * i * page_size ... (max_pages entries). */
+typedef struct hif4x_kv_batch {
+  const int *cu_new, *kv_len, *pages;
+  int sequences, max_pages;
+  int64_t ld_pages;
+} hif4x_kv_batch;
+
+/* New K and V rows into their places (rows x kv_heads x head_dim, unit inner
+ * stride, strides in elements, dtype HIF4X_DT_BF16 or HIF4X_DT_F32), by the
+ * searched encode of hif4x_convert, bit for bit.  Rows of no sequence and
+ * rows of a negative position are skipped.  Two rows of one call must not
+ * have the same place. */
+int hif4x_kv_append(const hif4x_kv_cache *kv, const hif4x_kv_batch *batch, const void *k, int64_t k_ld_row,
+                    int64_t k_ld_head, const void *v, int64_t v_ld_row, int64_t v_ld_head, int dtype, int64_t rows,
+                    void *stream);
+
+/* The values of the batch's rows (those that hif4x_kv_append writes), dense
+ * (rows, kv_heads, head_dim) of dtype HIF4X_DT_BF16 or HIF4X_DT_F32 (both
+ * exact), 16-byte aligned.  Rows that have no place are left as they were. */
+int hif4x_kv_read(const hif4x_kv_cache *kv, const hif4x_kv_batch *batch, int64_t rows, void *k, void *v, int dtype,
+                  void *stream);
+
+/* ---- serving: attention over the cache (csrc/paged_attention.cu) -------- */
+
+/* o = sum_t softmax_t(scale q.k_t) v_t for every new row and query head over
+ * the keys its position p = kv_len - new rows + j sees: t <= p and, with
+ * window > 0, t > p - window or t < sinks.  Query head h reads key head
+ * h / (q_heads / kv_heads).  A row that sees nothing gives 0.  q, out: rows x
+ * q_heads x head_dim bf16, strides in elements, multiples of 8, 16-byte
+ * aligned; rows of no sequence are left as they were.  max_new: about how
+ * many new rows a sequence has at most (it chooses the kernel; the result
+ * holds for any).  work: hif4x_paged_attention_work bytes, 16-byte aligned
+ * (NULL where that is 0), used until the call's kernels have run. */
+int hif4x_paged_attention_work(const hif4x_kv_cache *kv, const hif4x_kv_batch *batch, int q_heads, int64_t rows,
+                               int window, int sinks, int max_new, int64_t *bytes);
+int hif4x_paged_attention(const hif4x_kv_cache *kv, const hif4x_kv_batch *batch, const void *q, int64_t q_ld_row,
+                          int64_t q_ld_head, int q_heads, int64_t rows, float scale, int window, int sinks,
+                          int max_new, void *out, int64_t o_ld_row, int64_t o_ld_head, void *work,
+                          int64_t work_bytes, void *stream);
 
 #ifdef __cplusplus
 }
