@@ -55,34 +55,6 @@ struct Args {
   int *status;
 };
 
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(acc));
-}
-
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
-
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-      "[%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(addr));
-}
-
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -149,9 +121,9 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
                  "r"(a.tmem_cols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  asm volatile("tcgen05.fence::before_thread_sync;");
+  tc_fence_before();
   __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;");
+  tc_fence_after();
   const uint32_t tmem_a = *tmem_slot, tmem_d = tmem_a + STAGES * 32;   // A stages, then the accumulator
   bool ok = true;
 
@@ -171,14 +143,13 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t idesc =
-          (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(a.nt >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+      const uint32_t idesc = idesc_bf16((uint32_t)a.nt, 0);
       for (int i = 0; i < steps; i++) {
         const int s = i % STAGES, ph = (i / STAGES) & 1;
         ok = mbar_wait_limit(&full_x[s], ph, SPIN_LIMIT, a.status) &&
              mbar_wait_limit(&full_a[s], ph, SPIN_LIMIT, a.status);
         if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;");
+        tc_fence_after();
         const uint32_t xb = smem_u32(sx + s * x_bytes);
 #pragma unroll
         for (int j = 0; j < 4; j++)
@@ -241,11 +212,11 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
           ok = mbar_wait_limit(&empty[s], ((i / STAGES) - 1) & 1, SPIN_LIMIT, a.status);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;");
+          tc_fence_after();
         }
         tmem_st32(tmem_a + lanes + s * 32, v);
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        asm volatile("tcgen05.fence::before_thread_sync;");
+        tmem_wait_st();
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&full_a[s]);
       }
@@ -257,13 +228,13 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
     // ---- the accumulator to shared memory, [x row][row of W], over the x stages
     ok = mbar_wait_limit(done, 0, SPIN_LIMIT, a.status);
     __syncwarp();
-    asm volatile("tcgen05.fence::after_thread_sync;");
+    tc_fence_after();
     float *part = reinterpret_cast<float *>(sx);
     for (int n = wg * 16; n < a.nt; n += 32) {
       uint32_t d[16];
       if (steps > 0) {
         tmem_ld16(tmem_d + lanes + n, d);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        tmem_wait_ld();
       } else {
 #pragma unroll
         for (int k = 0; k < 16; k++) d[k] = 0u;
@@ -272,11 +243,11 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
       for (int k = 0; k < 16; k++) part[(n + k) * BM + r] = __uint_as_float(d[k]);
     }
   }
-  asm volatile("tcgen05.fence::before_thread_sync;");
+  tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     __syncwarp();
-    asm volatile("tcgen05.fence::after_thread_sync;");
+    tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_a), "r"(a.tmem_cols));
   }
   if (ranks > 1) cluster_sync();

@@ -24,6 +24,7 @@
 // meet in shared memory, the shares of one (sequence, key head) in a second
 // kernel that adds them in order (the result does not depend on timing).
 #include <algorithm>
+#include <cmath>
 
 #include "common.cuh"
 #include "hif4_bits.cuh"
@@ -41,6 +42,7 @@ struct AttendArgs {
   int group;                  // query heads per key head
   float scale;                // times log2(e)
   int window, sinks;          // window 0: all keys
+  int most_rows;              // attend_rows_kernel: sequences of up to so many rows; attend_tiles_kernel: of more
   int splits;
   float *part;                // (splits, rows, q heads, dh) sums, then (splits, rows, q heads) (reference, weight)
   float2 *part_ml;
@@ -142,6 +144,7 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(const AttendArgs a) {
   const int old = c.kv_len[s] - n_new;   // position of the first new row
   const int *pages = c.pages + s * c.ld_pages;
   const int64_t rows = (int64_t)n_new * a.group;
+  if (rows > a.most_rows) return;
 
   for (int64_t r0 = 0; r0 < rows; r0 += ROWS) {
     const int64_t r1 = min(rows, r0 + ROWS);
@@ -371,6 +374,440 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(const AttendArgs a) {
   }
 }
 
+// ---------------------------------------------------------------- many rows
+// attend_tiles_kernel (prefill chunks) is bound by the tensor cores, the
+// exponentials and the instructions around them.  A CTA takes 256 rows
+// (token, query head) of one key head as two tiles of 128 and walks the keys
+// 128 at a time:
+//   warps 0-3, 4-7  softmax of tile 0 and 1: a thread is one row; S from
+//                   tensor memory, weights back as bf16 pairs over S, where
+//                   the second product reads its A operand
+//   warp 8          one lane issues both products (tcgen05.mma kind::f16):
+//                   S = Q K^T (K-major K) and O += P V (V as it lies, keys by
+//                   dims: an MN-major B operand, so nothing is transposed)
+//   warps 12-15     decode the packed K and V tiles to bf16 in shared memory,
+//                   two stages each, words one half step ahead in registers
+// While one tile's softmax runs, the tensor core works on the other tile.
+// S and P of a tile share columns (S0 S1 O0 O1 fill the 512 columns at dh
+// 128), so S of the next step waits for the second product of this one.  The
+// softmax reference moves as in attend_rows_kernel, only past 2^8; then the
+// row's O is rescaled in tensor memory by the softmax warp itself: the
+// product that reads it next waits for this step's weights anyway.
+namespace tiles {
+
+using namespace tc;
+
+constexpr int THREADS = 512, KEYS = 128, ROWS = 256;
+
+template <int DH>
+struct Cfg {
+  static constexpr int TILE = 128 * DH * 2;                 // bytes of a 128-row bf16 tile
+  static constexpr int PANEL = 128 * 128;                   // 64 dims of it
+  static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE;   // two Q tiles, two stages of K and of V
+  static constexpr int BARS = 6 * TILE;
+  static constexpr int SMEM = BARS + 256 + 1024;
+};
+
+// keys a 16-byte code chunk of a warp lands on: lane -> (key of the run, chunk of 32 dims)
+template <int DH>
+struct Loader {
+  static constexpr int CPR = DH / 32;          // chunks per row; also steps per 32 keys
+  static constexpr int KPI = 32 / CPR;         // keys per step
+  uint4 w[CPR];
+  uint32_t m[CPR], have;                       // have: bit per step
+
+  // words of keys [key0 + 32 warp, + 32); pg: page ids of its two 16-key blocks (-1: none)
+  __device__ __forceinline__ void load(const CacheArgs &c, int which, int kh, int key_first, const int (&pg)[2],
+                                       int last, int lane) {
+    const int ch = lane >> 3;
+    have = 0;
+#pragma unroll
+    for (int it = 0; it < CPR; it++) {
+      const int k = it * KPI + (lane & 7) + (CPR == 2 ? 8 * (ch >> 1) : 0);
+      const int key = key_first + k, page = pg[(it * KPI) >> 4];
+      if (page >= 0 && key <= last) {
+        const int64_t row = ((int64_t)page * c.heads + kh) * c.page_size + (key & (c.page_size - 1));
+        const int cc = CPR == 4 ? ch : ch & 1;
+        w[it] = __ldg(reinterpret_cast<const uint4 *>(c.codes[which] + row * (DH / 2)) + cc);
+        m[it] = __ldg(c.meta[which] + row * (DH / 64) + (CPR == 4 ? cc >> 1 : 0));
+        have |= 1u << it;
+      }
+    }
+  }
+  // decoded into a tile: panel of 64 dims, key rows of 128 bytes, 16-byte chunk q at q ^ (key & 7)
+  __device__ __forceinline__ void store(uint8_t *tile, int warp, int lane) const {
+    const int ch = lane >> 3;
+#pragma unroll
+    for (int it = 0; it < CPR; it++) {
+      const int key = warp * 32 + it * KPI + (lane & 7) + (CPR == 2 ? 8 * (ch >> 1) : 0);
+      uint8_t *row = tile + (CPR == 4 ? (ch >> 1) * Cfg<DH>::PANEL : 0) + key * 128;
+      const bool ok = (have >> it) & 1u;
+      const uint32_t sf2 = hif4_sf2(m[it]);
+      const uint32_t ww[4] = {w[it].x, w[it].y, w[it].z, w[it].w};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int q = (ch & 1) * 4 + j;   // sub-block of the group = 16-byte chunk of the panel row
+        uint32_t o[4];
+        hif4_decode8(ww[j], m[it], sf2, q, o);
+        *reinterpret_cast<uint4 *>(row + ((q ^ (key & 7)) << 4)) =
+            ok ? make_uint4(o[0], o[1], o[2], o[3]) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+};
+
+// log2 weights of 32 columns: p = 2^(s scale - ref), summed and packed
+__device__ __forceinline__ void weights32(const uint32_t (&s)[32], float scale, float ref, float &sum, uint32_t *p) {
+  float a0 = 0.0f, a1 = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 16; j++) {
+    const float x = ex2(fmaf(__uint_as_float(s[2 * j]), scale, -ref));
+    const float y = ex2(fmaf(__uint_as_float(s[2 * j + 1]), scale, -ref));
+    a0 += x;
+    a1 += y;
+    p[j] = pack_bf16(x, y);
+  }
+  sum += a0 + a1;
+}
+
+template <int DH>
+__global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendArgs a, int flip) {
+  using C = Cfg<DH>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t *kfull = reinterpret_cast<uint64_t *>(smem + C::BARS), *kempty = kfull + 2, *vfull = kempty + 2;
+  uint64_t *vempty = vfull + 2, *sfull = vempty + 2, *pfull = sfull + 2, *odone = pfull + 2;
+  uint64_t *drain = odone + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+  int *found = reinterpret_cast<int *>(tmem_slot + 1);          // sequence, tile
+  uint8_t *hidden = reinterpret_cast<uint8_t *>(found + 2);     // [4 steps][4 warps]: 16-key blocks without a page
+  const CacheArgs &c = a.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kh = blockIdx.y, split = blockIdx.z;
+
+  // ---- which sequence and tile: the tiles of all sequences counted off, the last ones first
+  // (they see the most keys)
+  if (warp == 0) {
+    int left = blockIdx.x, seq = -1, tile = 0;
+    for (int b0 = 0; b0 < c.B && seq < 0; b0 += 32) {
+      const int b = b0 + lane;
+      const int64_t r = b < c.B ? (int64_t)max(0, c.cu_new[b + 1] - c.cu_new[b]) * a.group : 0;
+      const int n = r > a.most_rows ? (int)((r + ROWS - 1) / ROWS) : 0;
+      int sum = n;
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, sum, x);
+        if (lane >= x) sum += y;
+      }
+      const unsigned in = __ballot_sync(0xffffffffu, left < sum);
+      if (in) {
+        const int l = __ffs(in) - 1;
+        const int upto = __shfl_sync(0xffffffffu, sum, l);
+        seq = b0 + l;
+        tile = upto - 1 - left;
+      } else {
+        left -= __shfl_sync(0xffffffffu, sum, 31);
+      }
+    }
+    if (lane == 0) {
+      found[0] = seq;
+      found[1] = tile;
+      for (int i = 0; i < 2; i++) {
+        mbar_init(&kfull[i], 4);
+        mbar_init(&kempty[i], 1);
+        mbar_init(&vfull[i], 4);
+        mbar_init(&vempty[i], 1);
+        mbar_init(&sfull[i], 1);
+        mbar_init(&pfull[i], 4);
+        mbar_init(&odone[i], 1);
+      }
+      mbar_init(drain, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+  }
+  __syncthreads();
+  const int seq = found[0];
+  if (seq < 0) return;
+  if (warp == 8) {
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  const int cu0 = c.cu_new[seq], n_new = c.cu_new[seq + 1] - cu0, old = c.kv_len[seq] - n_new;
+  const int64_t rows = (int64_t)n_new * a.group, r0 = (int64_t)found[1] * ROWS;
+  const int tiles_here = rows - r0 > 128 ? 2 : 1;
+  const int64_t r1 = min(rows, r0 + ROWS);
+  const int p_lo = old + (int)(r0 / a.group), p_top = old + (int)((r1 - 1) / a.group);
+  const int64_t room = (int64_t)c.most << c.page_shift;
+  int p_hi = p_top;
+  if (p_hi >= room) {
+    if (threadIdx.x == 0) atomicExch(c.status, HIF4X_BAD_PAGE);
+    p_hi = (int)(room - 1);
+  }
+  const KeyTiles kt(min(max(p_lo, 0), p_hi), p_hi, a.window, a.sinks, KEYS);
+  const int per = (kt.n + a.splits - 1) / a.splits;
+  const int first = min(kt.n, split * per), n = min(kt.n, first + per) - first;   // steps of this CTA
+
+  // ---- Q into shared memory (K-major panels of 64 dims, 128-byte swizzle)
+  for (int e = threadIdx.x; e < tiles_here * 128 * (DH / 8); e += THREADS) {
+    const int r = e / (DH / 8), q = e % (DH / 8);
+    const int64_t rr = r0 + r, token = (int64_t)cu0 + rr / a.group;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (rr < r1 && token >= 0 && token < c.rows) {
+      x = __ldg(reinterpret_cast<const uint4 *>(a.q + token * a.q_row + (kh * a.group + (int)(rr % a.group)) * a.q_head) + q);
+      if (flip) {
+        x.x ^= 0x80008000u;
+        x.y ^= 0x80008000u;
+        x.z ^= 0x80008000u;
+        x.w ^= 0x80008000u;
+      }
+    }
+    *reinterpret_cast<uint4 *>(smem + C::Q + (r >> 7) * C::TILE + (q >> 3) * C::PANEL + (r & 127) * 128 +
+                               (((q & 7) ^ (r & 7)) << 4)) = x;
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  bool ok = true;
+
+  if (warp >= 12) {
+    // ---- decode
+    const int w = warp - 12;
+    const int *pages = c.pages + seq * c.ld_pages;
+    const int last = p_hi;
+    Loader<DH> kb, vb;
+    int pg[2];
+    auto look = [&](int i) {   // page ids of this warp's 32 keys of step i
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int key = kt.key0(first + i, KEYS) + w * 32 + h * 16;
+        pg[h] = -1;
+        if (i < n && key <= last) {
+          const int p = __ldg(pages + (key >> c.page_shift));
+          if (p >= 0 && p < c.num_pages) pg[h] = p;
+          else if (lane == 0) atomicExch(c.status, HIF4X_BAD_PAGE);
+        }
+      }
+    };
+    auto key_of = [&](int i) { return kt.key0(first + i, KEYS) + w * 32; };
+    int now[2], nxt[2];
+    look(0);
+    now[0] = pg[0];
+    now[1] = pg[1];
+    if (n > 0) {
+      kb.load(c, 0, kh, key_of(0), now, last, lane);
+      vb.load(c, 1, kh, key_of(0), now, last, lane);
+    }
+    look(1);
+    nxt[0] = pg[0];
+    nxt[1] = pg[1];
+    for (int i = 0; i < n && ok; i++) {
+      const int s = i & 1, ph = ((i >> 1) - 1) & 1;
+      if (i >= 2) ok = mbar_wait_limit(&kempty[s], ph, SPIN_LIMIT, c.status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      kb.store(smem + C::K + s * C::TILE, w, lane);
+      if (lane == 0) hidden[(i & 3) * 4 + w] = (uint8_t)((now[0] < 0 ? 1 : 0) | (now[1] < 0 ? 2 : 0));
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kfull[s]);
+      look(i + 2);
+      if (i + 1 < n) kb.load(c, 0, kh, key_of(i + 1), nxt, last, lane);
+      if (i >= 2) ok = mbar_wait_limit(&vempty[s], ph, SPIN_LIMIT, c.status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      vb.store(smem + C::V + s * C::TILE, w, lane);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&vfull[s]);
+      if (i + 1 < n) vb.load(c, 1, kh, key_of(i + 1), nxt, last, lane);
+      now[0] = nxt[0];
+      now[1] = nxt[1];
+      nxt[0] = pg[0];
+      nxt[1] = pg[1];
+    }
+  } else if (warp == 8) {
+    // ---- both products
+    if (lane == 0 && n > 0) {
+      const uint32_t base = smem_u32(smem);
+      auto qk = [&](int t, int i) {
+        const uint32_t qa = base + C::Q + t * C::TILE, kb = base + C::K + (i & 1) * C::TILE;
+#pragma unroll
+        for (int j = 0; j < DH / 16; j++) {
+          const uint32_t off = (j >> 2) * C::PANEL + (j & 3) * 32;
+          mma_f16_ss(tmem + t * 128, smem_desc(qa + off, 16u, 1024u, 2u), smem_desc(kb + off, 16u, 1024u, 2u),
+                     idesc_bf16(KEYS, 0), j > 0 ? 1u : 0u);
+        }
+        mma_commit(&sfull[t]);
+        if (t == tiles_here - 1) mma_commit(&kempty[i & 1]);
+      };
+      auto pv = [&](int t, int i) {
+        const uint32_t va = base + C::V + (i & 1) * C::TILE;
+#pragma unroll
+        for (int j = 0; j < KEYS / 16; j++)
+          mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + j * 8, smem_desc(va + j * 2048, C::PANEL, 1024u, 2u),
+                     idesc_bf16(DH, 1), (i > 0 || j > 0) ? 1u : 0u);
+        mma_commit(&odone[t]);
+        if (t == tiles_here - 1) mma_commit(&vempty[i & 1]);
+      };
+      ok = mbar_wait_limit(&kfull[0], 0, SPIN_LIMIT, c.status);
+      tc_fence_after();
+      for (int t = 0; t < tiles_here && ok; t++) qk(t, 0);
+      for (int i = 0; i < n && ok; i++) {
+        for (int t = 0; t < tiles_here && ok; t++) {
+          ok = mbar_wait_limit(&vfull[i & 1], (i >> 1) & 1, SPIN_LIMIT, c.status) &&
+               mbar_wait_limit(&pfull[t], i & 1, SPIN_LIMIT, c.status);
+          if (!ok) break;
+          tc_fence_after();
+          pv(t, i);
+          if (i + 1 < n) {
+            ok = mbar_wait_limit(&kfull[(i + 1) & 1], ((i + 1) >> 1) & 1, SPIN_LIMIT, c.status) &&
+                 mbar_wait_limit(&odone[t], i & 1, SPIN_LIMIT, c.status);
+            if (!ok) break;
+            tc_fence_after();
+            qk(t, i + 1);
+          }
+        }
+      }
+      mma_commit(drain);   // every issued product has finished before tensor memory is released
+      mbar_wait_limit(drain, 0, SPIN_LIMIT, c.status);
+    }
+    __syncwarp();
+  } else if (warp < 8) {
+    // ---- softmax: this thread's row
+    const int t = warp >> 2;
+    const int r = t * 128 + (warp & 3) * 32 + lane;
+    const int64_t rr = r0 + r;
+    if (t < tiles_here) {
+      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
+      const int p = rr < r1 ? old + (int)(rr / a.group) : -1;
+      // the least and the last position of this tile's rows
+      const int t_lo = old + (int)((r0 + t * 128) / a.group);
+      const int t_hi = old + (int)((min(r1, r0 + t * 128 + 128) - 1) / a.group);
+      float ref = -INFINITY, sum = 0.0f;
+      for (int i = 0; i < n; i++) {
+        ok = mbar_wait_limit(&sfull[t], i & 1, SPIN_LIMIT, c.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const int key0 = kt.key0(first + i, KEYS);
+        const uint32_t hid = *reinterpret_cast<const uint32_t *>(hidden + (i & 3) * 4);
+        const bool all = key0 + KEYS - 1 <= t_lo &&
+                         (a.window == 0 || key0 > t_hi - a.window || key0 + KEYS - 1 < a.sinks) && hid == 0;
+        uint32_t s[32];
+        // visible columns: j <= hi and (j > lo or j < sk), 16-key blocks with a page
+        const int hi = p - key0, lo = a.window ? p - a.window - key0 : -1, sk = a.sinks - key0;
+        auto mask = [&](int c0) {
+#pragma unroll
+          for (int j = 0; j < 32; j++) {
+            const int col = c0 + j;
+            const bool see = col <= hi && (col > lo || col < sk) && !((hid >> (c0 / 32 * 8 + j / 16)) & 1u);
+            s[j] = see ? s[j] : 0xff800000u;
+          }
+        };
+        float m = -INFINITY;
+#pragma unroll
+        for (int c0 = 0; c0 < KEYS; c0 += 32) {
+          tmem_ld32(ts + c0, s);
+          tmem_wait_ld();
+          if (!all) mask(c0);
+#pragma unroll
+          for (int j = 0; j < 32; j++) m = fmaxf(m, __uint_as_float(s[j]));
+        }
+        m *= a.scale;
+        if (__any_sync(0xffffffffu, m > ref + kLazy)) {
+          const float to_ref = fmaxf(m, ref);
+          const float f = ref == -INFINITY ? 0.0f : ex2(ref - to_ref);
+          ref = to_ref;
+          sum *= f;
+          if (i > 0) {
+#pragma unroll 1
+            for (int c0 = 0; c0 < DH; c0 += 32) {
+              tmem_ld32(to + c0, s);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; j++) s[j] = __float_as_uint(__uint_as_float(s[j]) * f);
+              tmem_st32(to + c0, s);
+            }
+          }
+        }
+        const float base = ref == -INFINITY ? 0.0f : ref;
+        uint32_t w[32];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+          for (int c0 = 0; c0 < 64; c0 += 32) {
+            tmem_ld32(ts + h * 64 + c0, s);
+            tmem_wait_ld();
+            if (!all) mask(h * 64 + c0);
+            weights32(s, a.scale, base, sum, w + c0 / 2);
+          }
+          tmem_st32(ts + h * 32, w);   // over S columns that have been read
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pfull[t]);
+      }
+      if (n > 0 && ok) {
+        ok = mbar_wait_limit(&odone[t], (n - 1) & 1, SPIN_LIMIT, c.status);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+      }
+      const int64_t token = (int64_t)cu0 + rr / a.group;
+      const bool mine = rr < r1 && token >= 0 && token < c.rows;
+      const int head = kh * a.group + (int)(rr % a.group);
+      const int64_t at = ((int64_t)split * c.rows + token) * (c.heads * a.group) + head;
+      const float inv = a.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+      if (a.splits > 1 && mine) a.part_ml[at] = make_float2(ref, sum);
+#pragma unroll 1
+      for (int c0 = 0; c0 < DH; c0 += 32) {
+        uint32_t o[32];
+        if (n > 0) {
+          tmem_ld32(to + c0, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; j++) o[j] = 0u;
+        }
+        if (!mine) continue;
+        if (a.splits > 1) {
+          float4 *dst = reinterpret_cast<float4 *>(a.part + at * DH + c0);
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]),
+                                 __uint_as_float(o[4 * j + 3]));
+        } else {
+          uint4 *dst = reinterpret_cast<uint4 *>(a.out + token * a.o_row + head * a.o_head + c0);
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            uint32_t x[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+              x[k] = sum == 0.0f ? 0u
+                                 : pack_bf16(__uint_as_float(o[8 * j + 2 * k]) * inv,
+                                             __uint_as_float(o[8 * j + 2 * k + 1]) * inv);
+            dst[j] = make_uint4(x[0], x[1], x[2], x[3]);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+}  // namespace tiles
+
 // The shares of a (row, query head), added in their order: a warp each.
 template <int DH>
 __global__ void __launch_bounds__(128) attend_join_kernel(const AttendArgs a) {
@@ -415,21 +852,63 @@ static int attend_splits(int sms, int64_t lanes, int64_t keys, int64_t outputs) 
 
 // How a call is carried out: from its sizes alone.
 struct AttendPlan {
-  int splits;
+  bool rows, tiles;          // the kernels that run
+  int most_rows;             // rows of a sequence up to which the first one takes it
+  int grid_tiles, splits;
   int64_t part_floats, work_bytes;
 };
 
+// Sequences of up to 16 rows (new tokens x query heads of a key head) go to
+// attend_rows_kernel, others to attend_tiles_kernel.  Only the device knows
+// the lengths: where max_new allows for more than 16 rows both kernels run and
+// each passes over the other's sequences, except that a single sequence is the
+// tiles kernel's alone.
 static int attend_plan(const hif4x_kv_cache *kv, const hif4x_kv_batch *b, int q_heads, int64_t rows, int window,
                        int sinks, int max_new, AttendPlan *p) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return HIF4X_ERR_LAUNCH;
   const int sms = tc::device_sms(dev);
   if (sms <= 0) return HIF4X_ERR_LAUNCH;
+  const int group = q_heads / kv->kv_heads;
+  const int64_t B = b->sequences, H = kv->kv_heads;
   int64_t keys = (int64_t)b->max_pages * kv->page_size;
   if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + max_new + sinks + 32);
-  p->splits = attend_splits(sms, (int64_t)b->sequences * kv->kv_heads, keys, rows * q_heads * kv->head_dim);
+  p->tiles = (int64_t)max_new * group > 16;
+  p->rows = !p->tiles || B > 1;
+  p->most_rows = !p->tiles ? INT32_MAX : B > 1 ? 16 : 0;
+  p->grid_tiles = 0;
+  if (p->tiles) {
+    const int64_t n = rows * group / tiles::ROWS + B;
+    if (n > INT32_MAX) return HIF4X_ERR_UNSUPPORTED;
+    p->grid_tiles = (int)n;
+    // shares of the keys: as many as fill the SMs once, four steps or more to each
+    const int64_t busy = std::max<int64_t>(1, rows * group / tiles::ROWS) * H;
+    p->splits = (int)std::max<int64_t>(
+        1, std::min<int64_t>({sms / busy, keys / (4 * tiles::KEYS), (int64_t(1) << 26) / (rows * q_heads * kv->head_dim), 64}));
+  } else {
+    p->splits = attend_splits(sms, B * H, keys, rows * q_heads * kv->head_dim);
+  }
   p->part_floats = p->splits > 1 ? (int64_t)p->splits * rows * q_heads * kv->head_dim : 0;
   p->work_bytes = p->splits > 1 ? p->part_floats * 4 + (int64_t)p->splits * rows * q_heads * 8 : 0;
+  return HIF4X_OK;
+}
+
+template <int DH>
+static int launch_tiles(AttendArgs a, int dev, const AttendPlan &p, cudaStream_t s) {
+  static std::once_flag once[tc::kMaxDevices];
+  static bool attr_ok[tc::kMaxDevices];
+  if (dev < 0 || dev >= tc::kMaxDevices) return HIF4X_ERR_LAUNCH;
+  std::call_once(once[dev], [dev] {
+    attr_ok[dev] = cudaFuncSetAttribute(tiles::attend_tiles_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        tiles::Cfg<DH>::SMEM) == cudaSuccess;
+  });
+  if (!attr_ok[dev]) return HIF4X_ERR_LAUNCH;
+  // the kernel compares unscaled scores, so its scale is positive: a negative one turns the queries' signs
+  const int flip = a.scale < 0.0f;
+  a.scale = std::max(std::fabs(a.scale), 1e-35f);
+  const dim3 grid((unsigned)p.grid_tiles, (unsigned)a.c.heads, (unsigned)p.splits);
+  tiles::attend_tiles_kernel<DH><<<grid, tiles::THREADS, tiles::Cfg<DH>::SMEM, s>>>(a, flip);
+  HIF4X_CHECK_LAUNCH();
   return HIF4X_OK;
 }
 
@@ -489,17 +968,26 @@ extern "C" int hif4x_paged_attention(const hif4x_kv_cache *kv, const hif4x_kv_ba
   a.splits = p.splits;
   a.part = static_cast<float *>(work);
   a.part_ml = reinterpret_cast<float2 *>(static_cast<float *>(work) + p.part_floats);
+  a.most_rows = p.most_rows;
   cudaStream_t s = (cudaStream_t)stream;
-  const dim3 grid((unsigned)batch->sequences, (unsigned)kv->kv_heads, (unsigned)p.splits);
-  const bool two = (int64_t)max_new * a.group > 8;
-  if (kv->head_dim == 128) {
-    if (two) attend_rows_kernel<128, 2><<<grid, 128, 0, s>>>(a);
-    else attend_rows_kernel<128, 1><<<grid, 128, 0, s>>>(a);
-  } else {
-    if (two) attend_rows_kernel<64, 2><<<grid, 128, 0, s>>>(a);
-    else attend_rows_kernel<64, 1><<<grid, 128, 0, s>>>(a);
+  if (p.tiles) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return HIF4X_ERR_LAUNCH;
+    st = kv->head_dim == 128 ? launch_tiles<128>(a, dev, p, s) : launch_tiles<64>(a, dev, p, s);
+    if (st != HIF4X_OK) return st;
   }
-  HIF4X_CHECK_LAUNCH();
+  if (p.rows) {
+    const dim3 grid((unsigned)batch->sequences, (unsigned)kv->kv_heads, (unsigned)p.splits);
+    const bool two = (int64_t)max_new * a.group > 8;
+    if (kv->head_dim == 128) {
+      if (two) attend_rows_kernel<128, 2><<<grid, 128, 0, s>>>(a);
+      else attend_rows_kernel<128, 1><<<grid, 128, 0, s>>>(a);
+    } else {
+      if (two) attend_rows_kernel<64, 2><<<grid, 128, 0, s>>>(a);
+      else attend_rows_kernel<64, 1><<<grid, 128, 0, s>>>(a);
+    }
+    HIF4X_CHECK_LAUNCH();
+  }
   if (p.splits > 1) {
     const unsigned blocks = (unsigned)((rows * q_heads + 3) / 4);
     if (kv->head_dim == 128) attend_join_kernel<128><<<blocks, 128, 0, s>>>(a);
