@@ -40,17 +40,28 @@ constexpr uint32_t kNeg136 = 0xc308c308u;   // bf16 pair -136
 // top of a bf16 significand, so its exponent is rebased by one addition
 __device__ __forceinline__ uint32_t hif4_sf2(uint32_t meta) { return (meta & 0xffu) * 0x00200020u + 0x26802680u; }
 
-// The scales of sub-block i (8 elements): quad 0 and quad 1, each in both halves.
-__device__ __forceinline__ void hif4_scales(uint32_t meta, uint32_t sf2, int i, uint32_t &s0, uint32_t &s1) {
-  const uint32_t b = ((meta >> (8 + i)) & 1u) * 0x00800080u + sf2;
-  s0 = ((meta >> (16 + 2 * i)) & 1u) * 0x00800080u + b;
-  s1 = ((meta >> (17 + 2 * i)) & 1u) * 0x00800080u + b;
+// The lv bits of four sub-blocks i0 .. i0 + 3 of a group: bit j of l2, bits 2j
+// and 2j + 1 of l3.
+struct Hif4Levels {
+  uint32_t l2, l3;
+  __device__ __forceinline__ Hif4Levels(uint32_t meta, int i0) : l2(meta >> (8 + i0)), l3(meta >> (16 + 2 * i0)) {}
+};
+// The scales of sub-block i0 + J (8 elements): quad 0 and quad 1, each in both
+// halves.  A bit is moved to both exponents' last place by a multiplication
+// (which leaves the ALU pipe, the busier one, to the masks).
+template <int J>
+__device__ __forceinline__ void hif4_scales(const Hif4Levels &l, uint32_t sf2, uint32_t &s0, uint32_t &s1) {
+  static_assert(J >= 0 && J < 4, "four sub-blocks");
+  const uint32_t b = (l.l2 & (1u << J)) * (0x00800080u >> J) + sf2;
+  s0 = (l.l3 & (1u << (2 * J))) * (0x00800080u >> (2 * J)) + b;
+  s1 = (l.l3 & (2u << (2 * J))) * (0x00800080u >> (2 * J + 1)) + b;
 }
 
-// Word of sub-block i -> four bf16 pairs in element order (0,1) (2,3) (4,5) (6,7).
-__device__ __forceinline__ void hif4_decode8(uint32_t w, uint32_t meta, uint32_t sf2, int i, uint32_t (&o)[4]) {
+// Word of sub-block i0 + J -> four bf16 pairs in element order (0,1) (2,3) (4,5) (6,7).
+template <int J>
+__device__ __forceinline__ void hif4_decode8(uint32_t w, const Hif4Levels &l, uint32_t sf2, uint32_t *o) {
   uint32_t s0, s1;
-  hif4_scales(meta, sf2, i, s0, s1);
+  hif4_scales<J>(l, sf2, s0, s1);
   const uint32_t z0 = bf16x2_mul(s0, kNeg136), z1 = bf16x2_mul(s1, kNeg136);
   const uint32_t lo = hif4_offset(w), hi = lo >> 4;
   // element 2p is nibble 2p (byte p of lo), element 2p + 1 the low nibble of byte p of hi
@@ -58,6 +69,33 @@ __device__ __forceinline__ void hif4_decode8(uint32_t w, uint32_t meta, uint32_t
   o[1] = bf16x2_fma((__byte_perm(lo, hi, 0x0501) & 0x000f000fu) | 0x43004300u, s0, z0);
   o[2] = bf16x2_fma((__byte_perm(lo, hi, 0x0602) & 0x000f000fu) | 0x43004300u, s1, z1);
   o[3] = bf16x2_fma((__byte_perm(lo, hi, 0x0703) & 0x000f000fu) | 0x43004300u, s1, z1);
+}
+
+// The same in the order (0,2) (4,6) (1,3) (5,7), two operations cheaper: the
+// even and the odd nibbles as bytes, a pair and its exponents by one permute.
+template <int J>
+__device__ __forceinline__ void hif4_decode8_even_odd(uint32_t w, const Hif4Levels &l, uint32_t sf2, uint32_t *o) {
+  uint32_t s0, s1;
+  hif4_scales<J>(l, sf2, s0, s1);
+  const uint32_t z0 = bf16x2_mul(s0, kNeg136), z1 = bf16x2_mul(s1, kNeg136);
+  const uint32_t c = hif4_offset(w), even = c & 0x0f0f0f0fu, odd = (c >> 4) & 0x0f0f0f0fu;
+  o[0] = bf16x2_fma(__byte_perm(even, 0x43434343u, 0x4140), s0, z0);
+  o[1] = bf16x2_fma(__byte_perm(even, 0x43434343u, 0x4342), s1, z1);
+  o[2] = bf16x2_fma(__byte_perm(odd, 0x43434343u, 0x4140), s0, z0);
+  o[3] = bf16x2_fma(__byte_perm(odd, 0x43434343u, 0x4342), s1, z1);
+}
+
+// Eight packed words and their meta word -> 64 values as bf16 pairs in order.
+__device__ __forceinline__ void hif4_decode64(const uint32_t (&w)[8], uint32_t meta, uint32_t (&v)[32]) {
+  const uint32_t sf2 = hif4_sf2(meta);
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const Hif4Levels l(meta, 4 * h);
+    hif4_decode8<0>(w[4 * h], l, sf2, v + 16 * h);
+    hif4_decode8<1>(w[4 * h + 1], l, sf2, v + 16 * h + 4);
+    hif4_decode8<2>(w[4 * h + 2], l, sf2, v + 16 * h + 8);
+    hif4_decode8<3>(w[4 * h + 3], l, sf2, v + 16 * h + 12);
+  }
 }
 
 // Where new row `token` of a batch belongs: its sequence (cu_new[s] <= token

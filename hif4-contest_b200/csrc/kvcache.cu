@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(128) read_kernel(const ReadArgs p) {
   const uint32_t w = reinterpret_cast<const uint32_t *>(c.codes[which])[unit * 8 + sub];
   const uint32_t m = c.meta[which][unit];
   uint32_t o[4];
-  hif4_decode8(w, m, hif4_sf2(m), sub, o);
+  hif4_decode8<0>(w, Hif4Levels(m, sub), hif4_sf2(m), o);
   const int64_t at = g * 8 + sub;
   if (p.dtype == HIF4X_DT_BF16) {
     static_cast<uint4 *>(p.out[which])[at] = make_uint4(o[0], o[1], o[2], o[3]);

@@ -192,21 +192,13 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
       for (int h = 0; h < 2; h++) {
         const int g = 2 * h + wg, i = 4 * b + g;   // group of the box, step
         if (i >= steps) break;
-        const uint32_t m = h ? m1 : m0, sf2 = hif4_sf2(m);
+        const uint32_t m = h ? m1 : m0;
         // 16-byte chunk c of row r lies at chunk c ^ (r & 7)
         const uint4 c0 = *reinterpret_cast<const uint4 *>(src + (((2 * g) ^ (r & 7)) << 4));
         const uint4 c1 = *reinterpret_cast<const uint4 *>(src + (((2 * g + 1) ^ (r & 7)) << 4));
         const uint32_t w[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
         uint32_t v[32];
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-          uint32_t o[4];
-          hif4_decode8(w[k], m, sf2, k, o);
-          v[4 * k] = o[0];
-          v[4 * k + 1] = o[1];
-          v[4 * k + 2] = o[2];
-          v[4 * k + 3] = o[3];
-        }
+        hif4_decode64(w, m, v);
         const int s = i % STAGES;
         if (i >= STAGES) {
           ok = mbar_wait_limit(&empty[s], ((i / STAGES) - 1) & 1, SPIN_LIMIT, a.status);

@@ -28,6 +28,7 @@
 
 #include "common.cuh"
 #include "hif4_bits.cuh"
+#include "hif4_enc.cuh"
 #include "kvcache.cuh"
 #include "sm100.cuh"
 
@@ -69,6 +70,14 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// hif4_scales of sub-block j, an index that unrolling makes constant
+__device__ __forceinline__ void scales_of(const Hif4Levels &l, uint32_t sf2, int j, uint32_t &s0, uint32_t &s1) {
+  if (j == 0) hif4_scales<0>(l, sf2, s0, s1);
+  else if (j == 1) hif4_scales<1>(l, sf2, s0, s1);
+  else if (j == 2) hif4_scales<2>(l, sf2, s0, s1);
+  else hif4_scales<3>(l, sf2, s0, s1);
 }
 
 // The 16-key tiles a run of positions [p_lo, p_hi] of one sequence can see:
@@ -223,12 +232,13 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(const AttendArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; e++) sc[nt][e] = 0.0f;
         const uint32_t sf0 = hif4_sf2(cur.km[0]), sf1 = hif4_sf2(cur.km[1]);
+        const int i0 = DH == 128 ? (q4 & 1) * 4 : q4 * 2;   // sub-block of the group
+        const Hif4Levels l0(cur.km[0], i0), l1(cur.km[1], i0);
 #pragma unroll
         for (int w = 0; w < KW; w++) {
-          const int i = (DH == 128 ? (q4 & 1) * 4 : q4 * 2) + w;   // sub-block of the group
           uint32_t a0, a1, b0, b1;
-          hif4_scales(cur.km[0], sf0, i, a0, a1);
-          hif4_scales(cur.km[1], sf1, i, b0, b1);
+          scales_of(l0, sf0, w, a0, a1);
+          scales_of(l1, sf1, w, b0, b1);
           const uint32_t s0 = __byte_perm(a0, a1, 0x5410), s1 = __byte_perm(b0, b1, 0x5410);
           const uint32_t z0 = bf16x2_mul(s0, kNeg136), z1 = bf16x2_mul(s1, kNeg136);
           const uint32_t x0 = hif4_offset(cur.k[0][w]), x1 = hif4_offset(cur.k[1][w]);
@@ -297,11 +307,10 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(const AttendArgs a) {
         for (int u = 0; u < 4; u++) vsf[u] = hif4_sf2(cur.vm[u]);
 #pragma unroll
         for (int w = 0; w < DH / 64; w++) {
-          const int i = DH == 128 ? (n8 & 3) * 2 + w : n8;   // sub-block of the group
           uint32_t sk[4][2], x[4];
 #pragma unroll
           for (int u = 0; u < 4; u++) {
-            hif4_scales(cur.vm[u], vsf[u], i, sk[u][0], sk[u][1]);
+            scales_of(Hif4Levels(cur.vm[u], DH == 128 ? (n8 & 3) * 2 : n8), vsf[u], w, sk[u][0], sk[u][1]);
             x[u] = hif4_offset(cur.v[u][w]);
           }
 #pragma unroll
@@ -434,40 +443,48 @@ struct Loader {
       }
     }
   }
-  // decoded into a tile: panel of 64 dims, key rows of 128 bytes, 16-byte chunk q at q ^ (key & 7)
+  // decoded into a tile: panel of 64 dims, key rows of 128 bytes, 16-byte chunk q at q ^ (key & 7); inside a
+  // chunk the dims stand as (0 2 4 6 1 3 5 7), as Q's do
   __device__ __forceinline__ void store(uint8_t *tile, int warp, int lane) const {
-    const int ch = lane >> 3;
+    const int ch = lane >> 3, q0 = (ch & 1) * 4;   // first sub-block of the group = 16-byte chunk of the panel row
 #pragma unroll
     for (int it = 0; it < CPR; it++) {
       const int key = warp * 32 + it * KPI + (lane & 7) + (CPR == 2 ? 8 * (ch >> 1) : 0);
       uint8_t *row = tile + (CPR == 4 ? (ch >> 1) * Cfg<DH>::PANEL : 0) + key * 128;
       const bool ok = (have >> it) & 1u;
-      const uint32_t sf2 = hif4_sf2(m[it]);
-      const uint32_t ww[4] = {w[it].x, w[it].y, w[it].z, w[it].w};
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int q = (ch & 1) * 4 + j;   // sub-block of the group = 16-byte chunk of the panel row
-        uint32_t o[4];
-        hif4_decode8(ww[j], m[it], sf2, q, o);
-        *reinterpret_cast<uint4 *>(row + ((q ^ (key & 7)) << 4)) =
-            ok ? make_uint4(o[0], o[1], o[2], o[3]) : make_uint4(0, 0, 0, 0);
-      }
+      const uint32_t mm = ok ? m[it] : 0u, sf2 = hif4_sf2(mm);
+      const Hif4Levels l(mm, q0);
+      const uint4 c = ok ? w[it] : make_uint4(0, 0, 0, 0);   // code 0 decodes to 0
+      uint32_t o[4];
+      hif4_decode8_even_odd<0>(c.x, l, sf2, o);
+      *reinterpret_cast<uint4 *>(row + ((q0 ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+      hif4_decode8_even_odd<1>(c.y, l, sf2, o);
+      *reinterpret_cast<uint4 *>(row + (((q0 + 1) ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+      hif4_decode8_even_odd<2>(c.z, l, sf2, o);
+      *reinterpret_cast<uint4 *>(row + (((q0 + 2) ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+      hif4_decode8_even_odd<3>(c.w, l, sf2, o);
+      *reinterpret_cast<uint4 *>(row + (((q0 + 3) ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   }
 };
 
-// log2 weights of 32 columns: p = 2^(s scale - ref), summed and packed
-__device__ __forceinline__ void weights32(const uint32_t (&s)[32], float scale, float ref, float &sum, uint32_t *p) {
-  float a0 = 0.0f, a1 = 0.0f;
+// weights of 32 columns: p = 2^(s scale - ref), summed (pairs of sums) and packed
+__device__ __forceinline__ void weights32(const uint32_t (&s)[32], u64 scale2, u64 nref2, u64 &sum2, uint32_t *p) {
 #pragma unroll
   for (int j = 0; j < 16; j++) {
-    const float x = ex2(fmaf(__uint_as_float(s[2 * j]), scale, -ref));
-    const float y = ex2(fmaf(__uint_as_float(s[2 * j + 1]), scale, -ref));
-    a0 += x;
-    a1 += y;
+    float x, y;
+    upk2(fma2(pk2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), scale2, nref2), x, y);
+    x = ex2(x);
+    y = ex2(y);
+    sum2 = add2(sum2, pk2(x, y));
     p[j] = pack_bf16(x, y);
   }
-  sum += a0 + a1;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 template <int DH>
@@ -564,7 +581,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
       }
     }
     *reinterpret_cast<uint4 *>(smem + C::Q + (r >> 7) * C::TILE + (q >> 3) * C::PANEL + (r & 127) * 128 +
-                               (((q & 7) ^ (r & 7)) << 4)) = x;
+                               (((q & 7) ^ (r & 7)) << 4)) =
+        make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.z, x.w, 0x5410), __byte_perm(x.x, x.y, 0x7632),
+                   __byte_perm(x.z, x.w, 0x7632));
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc_fence_before();
@@ -578,9 +597,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
     const int w = warp - 12;
     const int *pages = c.pages + seq * c.ld_pages;
     const int last = p_hi;
-    Loader<DH> kb, vb;
-    int pg[2];
-    auto look = [&](int i) {   // page ids of this warp's 32 keys of step i
+    // half step u: K (even) or V (odd) of step u / 2; the next one's words are on their way meanwhile
+    Loader<DH> cur, next;
+    auto look = [&](int i, int (&pg)[2]) {   // page ids of this warp's 32 keys of step i
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const int key = kt.key0(first + i, KEYS) + w * 32 + h * 16;
@@ -592,64 +611,54 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         }
       }
     };
-    auto key_of = [&](int i) { return kt.key0(first + i, KEYS) + w * 32; };
-    int now[2], nxt[2];
-    look(0);
-    now[0] = pg[0];
-    now[1] = pg[1];
-    if (n > 0) {
-      kb.load(c, 0, kh, key_of(0), now, last, lane);
-      vb.load(c, 1, kh, key_of(0), now, last, lane);
-    }
-    look(1);
-    nxt[0] = pg[0];
-    nxt[1] = pg[1];
-    for (int i = 0; i < n && ok; i++) {
-      const int s = i & 1, ph = ((i >> 1) - 1) & 1;
-      if (i >= 2) ok = mbar_wait_limit(&kempty[s], ph, SPIN_LIMIT, c.status);
+    int now[2], nxt[2];   // of the step being decoded, of the step after it
+    look(0, now);
+    look(1, nxt);
+    if (n > 0) cur.load(c, 0, kh, kt.key0(first, KEYS) + w * 32, now, last, lane);
+#pragma unroll 1
+    for (int u = 0; u < 2 * n; u++) {
+      const int i = u >> 1, v = u & 1, s = i & 1;
+      if (v == 0) {
+        next.load(c, 1, kh, kt.key0(first + i, KEYS) + w * 32, now, last, lane);
+        if (lane == 0) hidden[(i & 3) * 4 + w] = (uint8_t)((now[0] < 0 ? 1 : 0) | (now[1] < 0 ? 2 : 0));
+      } else if (i + 1 < n) {
+        next.load(c, 0, kh, kt.key0(first + i + 1, KEYS) + w * 32, nxt, last, lane);
+        now[0] = nxt[0];
+        now[1] = nxt[1];
+        look(i + 2, nxt);
+      }
+      if (i >= 2) ok = mbar_wait_limit((v ? vempty : kempty) + s, ((i >> 1) - 1) & 1, SPIN_LIMIT, c.status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      kb.store(smem + C::K + s * C::TILE, w, lane);
-      if (lane == 0) hidden[(i & 3) * 4 + w] = (uint8_t)((now[0] < 0 ? 1 : 0) | (now[1] < 0 ? 2 : 0));
+      cur.store(smem + (v ? C::V : C::K) + s * C::TILE, w, lane);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&kfull[s]);
-      look(i + 2);
-      if (i + 1 < n) kb.load(c, 0, kh, key_of(i + 1), nxt, last, lane);
-      if (i >= 2) ok = mbar_wait_limit(&vempty[s], ph, SPIN_LIMIT, c.status);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      vb.store(smem + C::V + s * C::TILE, w, lane);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&vfull[s]);
-      if (i + 1 < n) vb.load(c, 1, kh, key_of(i + 1), nxt, last, lane);
-      now[0] = nxt[0];
-      now[1] = nxt[1];
-      nxt[0] = pg[0];
-      nxt[1] = pg[1];
+      if (lane == 0) mbar_arrive((v ? vfull : kfull) + s);
+      cur = next;
     }
   } else if (warp == 8) {
     // ---- both products
     if (lane == 0 && n > 0) {
       const uint32_t base = smem_u32(smem);
+      // descriptors of the first K-substep; a step further is a constant in their address bits (16-byte units)
+      const uint64_t dq = smem_desc(base + C::Q, 16u, 1024u, 2u), dk = smem_desc(base + C::K, 16u, 1024u, 2u);
+      const uint64_t dv = smem_desc(base + C::V, C::PANEL, 1024u, 2u);
       auto qk = [&](int t, int i) {
-        const uint32_t qa = base + C::Q + t * C::TILE, kb = base + C::K + (i & 1) * C::TILE;
+        const uint64_t q = dq + t * (C::TILE >> 4), k = dk + (i & 1) * (C::TILE >> 4);
 #pragma unroll
         for (int j = 0; j < DH / 16; j++) {
-          const uint32_t off = (j >> 2) * C::PANEL + (j & 3) * 32;
-          mma_f16_ss(tmem + t * 128, smem_desc(qa + off, 16u, 1024u, 2u), smem_desc(kb + off, 16u, 1024u, 2u),
-                     idesc_bf16(KEYS, 0), j > 0 ? 1u : 0u);
+          const uint32_t off = ((j >> 2) * C::PANEL + (j & 3) * 32) >> 4;
+          mma_f16_ss(tmem + t * 128, q + off, k + off, idesc_bf16(KEYS, 0), j > 0 ? 1u : 0u);
         }
         mma_commit(&sfull[t]);
         if (t == tiles_here - 1) mma_commit(&kempty[i & 1]);
       };
       auto pv = [&](int t, int i) {
-        const uint32_t va = base + C::V + (i & 1) * C::TILE;
+        const uint64_t v = dv + (i & 1) * (C::TILE >> 4);
 #pragma unroll
         for (int j = 0; j < KEYS / 16; j++)
-          mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + j * 8, smem_desc(va + j * 2048, C::PANEL, 1024u, 2u),
-                     idesc_bf16(DH, 1), (i > 0 || j > 0) ? 1u : 0u);
+          mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + j * 8, v + j * (2048 >> 4), idesc_bf16(DH, 1),
+                     (i > 0 || j > 0) ? 1u : 0u);
         mma_commit(&odone[t]);
         if (t == tiles_here - 1) mma_commit(&vempty[i & 1]);
       };
@@ -688,7 +697,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
       // the least and the last position of this tile's rows
       const int t_lo = old + (int)((r0 + t * 128) / a.group);
       const int t_hi = old + (int)((min(r1, r0 + t * 128 + 128) - 1) / a.group);
-      float ref = -INFINITY, sum = 0.0f;
+      float ref = -INFINITY;
+      u64 sum2 = pk2(0.0f, 0.0f);
+#pragma unroll 1
       for (int i = 0; i < n; i++) {
         ok = mbar_wait_limit(&sfull[t], i & 1, SPIN_LIMIT, c.status);
         ok = __all_sync(0xffffffffu, ok);
@@ -698,32 +709,50 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         const uint32_t hid = *reinterpret_cast<const uint32_t *>(hidden + (i & 3) * 4);
         const bool all = key0 + KEYS - 1 <= t_lo &&
                          (a.window == 0 || key0 > t_hi - a.window || key0 + KEYS - 1 < a.sinks) && hid == 0;
-        uint32_t s[32];
-        // visible columns: j <= hi and (j > lo or j < sk), 16-key blocks with a page
-        const int hi = p - key0, lo = a.window ? p - a.window - key0 : -1, sk = a.sinks - key0;
-        auto mask = [&](int c0) {
-#pragma unroll
-          for (int j = 0; j < 32; j++) {
-            const int col = c0 + j;
-            const bool see = col <= hi && (col > lo || col < sk) && !((hid >> (c0 / 32 * 8 + j / 16)) & 1u);
-            s[j] = see ? s[j] : 0xff800000u;
-          }
-        };
+        uint32_t s[32], s1[32];
+        // the row's largest score; where not all keys are visible, hidden columns are -inf from here on
         float m = -INFINITY;
+        if (all) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < KEYS; c0 += 64) {
+            tmem_ld32(ts + c0, s);
+            tmem_ld32(ts + c0 + 32, s1);
+            tmem_wait_ld();
+            float x[4] = {m, m, m, m};
 #pragma unroll
-        for (int c0 = 0; c0 < KEYS; c0 += 32) {
-          tmem_ld32(ts + c0, s);
-          tmem_wait_ld();
-          if (!all) mask(c0);
+            for (int j = 0; j < 32; j += 4) {
+              x[0] = max3(x[0], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+              x[1] = max3(x[1], __uint_as_float(s[j + 2]), __uint_as_float(s[j + 3]));
+              x[2] = max3(x[2], __uint_as_float(s1[j]), __uint_as_float(s1[j + 1]));
+              x[3] = max3(x[3], __uint_as_float(s1[j + 2]), __uint_as_float(s1[j + 3]));
+            }
+            m = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          }
+        } else {
+          // visible columns: j <= hi and (j > lo or j < sk), 16-key blocks with a page
+          const int hi = p - key0, lo = a.window ? p - a.window - key0 : -1, sk = a.sinks - key0;
+#pragma unroll 1
+          for (int c0 = 0; c0 < KEYS; c0 += 32) {
+            tmem_ld32(ts + c0, s);
+            tmem_wait_ld();
+            const uint32_t hb = hid >> (c0 / 4);
 #pragma unroll
-          for (int j = 0; j < 32; j++) m = fmaxf(m, __uint_as_float(s[j]));
+            for (int j = 0; j < 32; j++) {
+              const int col = c0 + j;
+              const bool see = col <= hi && (col > lo || col < sk) && !((hb >> (j / 16)) & 1u);
+              s[j] = see ? s[j] : 0xff800000u;
+              m = fmaxf(m, __uint_as_float(s[j]));
+            }
+            tmem_st32(ts + c0, s);
+          }
+          tmem_wait_st();
         }
         m *= a.scale;
         if (__any_sync(0xffffffffu, m > ref + kLazy)) {
           const float to_ref = fmaxf(m, ref);
           const float f = ref == -INFINITY ? 0.0f : ex2(ref - to_ref);
           ref = to_ref;
-          sum *= f;
+          sum2 = mul2(sum2, pk2(f, f));
           if (i > 0) {
 #pragma unroll 1
             for (int c0 = 0; c0 < DH; c0 += 32) {
@@ -736,17 +765,16 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
           }
         }
         const float base = ref == -INFINITY ? 0.0f : ref;
-        uint32_t w[32];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-#pragma unroll
-          for (int c0 = 0; c0 < 64; c0 += 32) {
-            tmem_ld32(ts + h * 64 + c0, s);
-            tmem_wait_ld();
-            if (!all) mask(h * 64 + c0);
-            weights32(s, a.scale, base, sum, w + c0 / 2);
-          }
-          tmem_st32(ts + h * 32, w);   // over S columns that have been read
+        const u64 scale2 = pk2(a.scale, a.scale), nref2 = pk2(-base, -base);
+#pragma unroll 1
+        for (int c0 = 0; c0 < KEYS; c0 += 64) {
+          uint32_t w[32];
+          tmem_ld32(ts + c0, s);
+          tmem_ld32(ts + c0 + 32, s1);
+          tmem_wait_ld();
+          weights32(s, scale2, nref2, sum2, w);
+          weights32(s1, scale2, nref2, sum2, w + 16);
+          tmem_st32(ts + c0 / 2, w);   // over S columns that have been read
         }
         tmem_wait_st();
         tc_fence_before();
@@ -758,6 +786,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
+      float s_even, s_odd;
+      upk2(sum2, s_even, s_odd);
+      const float sum = s_even + s_odd;
       const int64_t token = (int64_t)cu0 + rr / a.group;
       const bool mine = rr < r1 && token >= 0 && token < c.rows;
       const int head = kh * a.group + (int)(rr % a.group);
@@ -775,12 +806,15 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
           for (int j = 0; j < 32; j++) o[j] = 0u;
         }
         if (!mine) continue;
+        // a chunk of eight dims stands as (0 2 4 6 1 3 5 7)
         if (a.splits > 1) {
           float4 *dst = reinterpret_cast<float4 *>(a.part + at * DH + c0);
 #pragma unroll
-          for (int j = 0; j < 8; j++)
-            dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]),
-                                 __uint_as_float(o[4 * j + 3]));
+          for (int j = 0; j < 8; j++) {
+            const int e = 8 * (j >> 1) + 2 * (j & 1);
+            dst[j] = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 4]), __uint_as_float(o[e + 1]),
+                                 __uint_as_float(o[e + 5]));
+          }
         } else {
           uint4 *dst = reinterpret_cast<uint4 *>(a.out + token * a.o_row + head * a.o_head + c0);
 #pragma unroll
@@ -789,8 +823,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
 #pragma unroll
             for (int k = 0; k < 4; k++)
               x[k] = sum == 0.0f ? 0u
-                                 : pack_bf16(__uint_as_float(o[8 * j + 2 * k]) * inv,
-                                             __uint_as_float(o[8 * j + 2 * k + 1]) * inv);
+                                 : pack_bf16(__uint_as_float(o[8 * j + k]) * inv, __uint_as_float(o[8 * j + k + 4]) * inv);
             dst[j] = make_uint4(x[0], x[1], x[2], x[3]);
           }
         }
