@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
   bool ok = true;
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       int i = 0;
       for (; i < steps; i++) {
         const int s = i % STAGES;
@@ -142,25 +142,25 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
         if (i > s) mbar_wait_limit(&full_x[s], ((i - 1 - s) / STAGES) & 1, SPIN_LIMIT, a.status);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t idesc = idesc_bf16((uint32_t)a.nt, 0);
+      const uint64_t dx = smem_desc(smem_u32(sx), 16u, 1024u, 2u);   // + 2 for 32 bytes further
       for (int i = 0; i < steps; i++) {
         const int s = i % STAGES, ph = (i / STAGES) & 1;
         ok = mbar_wait_limit(&full_x[s], ph, SPIN_LIMIT, a.status) &&
              mbar_wait_limit(&full_a[s], ph, SPIN_LIMIT, a.status);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t xb = smem_u32(sx + s * x_bytes);
+        const uint64_t x = dx + (uint32_t)(s * x_bytes >> 4);
 #pragma unroll
         for (int j = 0; j < 4; j++)
-          mma_f16_ts(tmem_d, tmem_a + s * 32 + j * 8, smem_desc(xb + 32u * j, 16u, 1024u, 2u), idesc,
-                     (i > 0 || j > 0) ? 1u : 0u);
+          mma_f16_ts(tmem_d, tmem_a + s * 32 + j * 8, x + 2 * j, idesc, (i > 0 || j > 0) ? 1u : 0u);
         mma_commit(&empty[s]);
       }
       mma_commit(done);
     }
   } else if (warp == 2) {
-    if (lane == 0) {
+    if (elect_one()) {
       const int boxes = (steps + 3) / 4;
       int i = 0;
       for (; i < boxes; i++) {

@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(const AttendArgs a) {
 //   warps 0-3, 4-7  softmax of tile 0 and 1: a thread is one row; S from
 //                   tensor memory, weights back as bf16 pairs over S, where
 //                   the second product reads its A operand
-//   warp 8          one lane issues both products (tcgen05.mma kind::f16):
+//   warps 8, 9      one lane each issues a tile's products (tcgen05.mma kind::f16):
 //                   S = Q K^T (K-major K) and O += P V (V as it lies, keys by
 //                   dims: an MN-major B operand, so nothing is transposed)
 //   warps 12-15     decode the packed K and V tiles to bf16 in shared memory,
@@ -493,9 +493,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t *kfull = reinterpret_cast<uint64_t *>(smem + C::BARS), *kempty = kfull + 2, *vfull = kempty + 2;
-  uint64_t *vempty = vfull + 2, *sfull = vempty + 2, *pfull = sfull + 2, *odone = pfull + 2;
+  uint64_t *vempty = vfull + 2, *sfull = vempty + 2, *pfull = sfull + 2, *odone = pfull + 4;
   uint64_t *drain = odone + 2;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 2);
   int *found = reinterpret_cast<int *>(tmem_slot + 1);          // sequence, tile
   uint8_t *hidden = reinterpret_cast<uint8_t *>(found + 2);     // [4 steps][4 warps]: 16-key blocks without a page
   const CacheArgs &c = a.c;
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
   // ---- which sequence and tile: the tiles of all sequences counted off, the last ones first
   // (they see the most keys)
   if (warp == 0) {
-    int left = blockIdx.x, seq = -1, tile = 0;
+    int left = blockIdx.x, seq = -1, tile = 0, two = 1;
     for (int b0 = 0; b0 < c.B && seq < 0; b0 += 32) {
       const int b = b0 + lane;
       const int64_t r = b < c.B ? (int64_t)max(0, c.cu_new[b + 1] - c.cu_new[b]) * a.group : 0;
@@ -522,6 +522,8 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         const int upto = __shfl_sync(0xffffffffu, sum, l);
         seq = b0 + l;
         tile = upto - 1 - left;
+        // 1 or 2 tiles of 128 rows
+        two = __shfl_sync(0xffffffffu, r, l) - (int64_t)tile * ROWS > 128 ? 2 : 1;
       } else {
         left -= __shfl_sync(0xffffffffu, sum, 31);
       }
@@ -531,14 +533,15 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
       found[1] = tile;
       for (int i = 0; i < 2; i++) {
         mbar_init(&kfull[i], 4);
-        mbar_init(&kempty[i], 1);
+        mbar_init(&kempty[i], two);
         mbar_init(&vfull[i], 4);
-        mbar_init(&vempty[i], 1);
+        mbar_init(&vempty[i], two);
         mbar_init(&sfull[i], 1);
         mbar_init(&pfull[i], 4);
+        mbar_init(&pfull[2 + i], 4);
         mbar_init(&odone[i], 1);
+        mbar_init(&drain[i], 1);
       }
-      mbar_init(drain, 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
   }
@@ -636,53 +639,54 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
       if (lane == 0) mbar_arrive((v ? vfull : kfull) + s);
       cur = next;
     }
-  } else if (warp == 8) {
-    // ---- both products
-    if (lane == 0 && n > 0) {
+  } else if (warp == 8 || warp == 9) {
+    // ---- both products of tile warp - 8
+    const int t = warp - 8;
+    if (t < tiles_here && n > 0 && elect_one()) {
       const uint32_t base = smem_u32(smem);
       // descriptors of the first K-substep; a step further is a constant in their address bits (16-byte units)
-      const uint64_t dq = smem_desc(base + C::Q, 16u, 1024u, 2u), dk = smem_desc(base + C::K, 16u, 1024u, 2u);
-      const uint64_t dv = smem_desc(base + C::V, C::PANEL, 1024u, 2u);
-      auto qk = [&](int t, int i) {
-        const uint64_t q = dq + t * (C::TILE >> 4), k = dk + (i & 1) * (C::TILE >> 4);
-#pragma unroll
-        for (int j = 0; j < DH / 16; j++) {
-          const uint32_t off = ((j >> 2) * C::PANEL + (j & 3) * 32) >> 4;
-          mma_f16_ss(tmem + t * 128, q + off, k + off, idesc_bf16(KEYS, 0), j > 0 ? 1u : 0u);
-        }
-        mma_commit(&sfull[t]);
-        if (t == tiles_here - 1) mma_commit(&kempty[i & 1]);
-      };
-      auto pv = [&](int t, int i) {
-        const uint64_t v = dv + (i & 1) * (C::TILE >> 4);
-#pragma unroll
-        for (int j = 0; j < KEYS / 16; j++)
-          mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + j * 8, v + j * (2048 >> 4), idesc_bf16(DH, 1),
-                     (i > 0 || j > 0) ? 1u : 0u);
-        mma_commit(&odone[t]);
-        if (t == tiles_here - 1) mma_commit(&vempty[i & 1]);
-      };
-      ok = mbar_wait_limit(&kfull[0], 0, SPIN_LIMIT, c.status);
-      tc_fence_after();
-      for (int t = 0; t < tiles_here && ok; t++) qk(t, 0);
-      for (int i = 0; i < n && ok; i++) {
-        for (int t = 0; t < tiles_here && ok; t++) {
-          ok = mbar_wait_limit(&vfull[i & 1], (i >> 1) & 1, SPIN_LIMIT, c.status) &&
-               mbar_wait_limit(&pfull[t], i & 1, SPIN_LIMIT, c.status);
+      const uint64_t dq = smem_desc(base + C::Q + t * C::TILE, 16u, 1024u, 2u);
+      const uint64_t dk = smem_desc(base + C::K, 16u, 1024u, 2u), dv = smem_desc(base + C::V, C::PANEL, 1024u, 2u);
+      const uint32_t d_s = tmem + t * 128, d_o = tmem + 256 + t * 128;
+#pragma unroll 1
+      for (int i = 0; i <= n; i++) {
+        if (i > 0) {   // O += P V of step i - 1, in two halves of 64 keys as the weights come
+          const int s = (i - 1) & 1;
+          const uint64_t v = dv + s * (C::TILE >> 4);
+          ok = mbar_wait_limit(&vfull[s], ((i - 1) >> 1) & 1, SPIN_LIMIT, c.status) &&
+               mbar_wait_limit(&pfull[t], s, SPIN_LIMIT, c.status);
           if (!ok) break;
           tc_fence_after();
-          pv(t, i);
-          if (i + 1 < n) {
-            ok = mbar_wait_limit(&kfull[(i + 1) & 1], ((i + 1) >> 1) & 1, SPIN_LIMIT, c.status) &&
-                 mbar_wait_limit(&odone[t], i & 1, SPIN_LIMIT, c.status);
-            if (!ok) break;
-            tc_fence_after();
-            qk(t, i + 1);
+#pragma unroll
+          for (int j = 0; j < KEYS / 32; j++)
+            mma_f16_ts(d_o, d_s + j * 8, v + j * (2048 >> 4), idesc_bf16(DH, 1), (i > 1 || j > 0) ? 1u : 0u);
+          ok = mbar_wait_limit(&pfull[2 + t], s, SPIN_LIMIT, c.status);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int j = KEYS / 32; j < KEYS / 16; j++)
+            mma_f16_ts(d_o, d_s + j * 8, v + j * (2048 >> 4), idesc_bf16(DH, 1), 1u);
+          mma_commit(&odone[t]);
+          mma_commit(&vempty[s]);
+        }
+        if (i < n) {   // S of step i, over the weights of step i - 1
+          const int s = i & 1;
+          const uint64_t k = dk + s * (C::TILE >> 4);
+          ok = mbar_wait_limit(&kfull[s], (i >> 1) & 1, SPIN_LIMIT, c.status) &&
+               (i == 0 || mbar_wait_limit(&odone[t], (i - 1) & 1, SPIN_LIMIT, c.status));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int j = 0; j < DH / 16; j++) {
+            const uint32_t off = ((j >> 2) * C::PANEL + (j & 3) * 32) >> 4;
+            mma_f16_ss(d_s, dq + off, k + off, idesc_bf16(KEYS, 0), j > 0 ? 1u : 0u);
           }
+          mma_commit(&sfull[t]);
+          mma_commit(&kempty[s]);
         }
       }
-      mma_commit(drain);   // every issued product has finished before tensor memory is released
-      mbar_wait_limit(drain, 0, SPIN_LIMIT, c.status);
+      mma_commit(&drain[t]);   // every issued product has finished before tensor memory is released
+      mbar_wait_limit(&drain[t], 0, SPIN_LIMIT, c.status);
     }
     __syncwarp();
   } else if (warp < 8) {
@@ -766,20 +770,23 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         }
         const float base = ref == -INFINITY ? 0.0f : ref;
         const u64 scale2 = pk2(a.scale, a.scale), nref2 = pk2(-base, -base);
-#pragma unroll 1
-        for (int c0 = 0; c0 < KEYS; c0 += 64) {
-          uint32_t w[32];
-          tmem_ld32(ts + c0, s);
-          tmem_ld32(ts + c0 + 32, s1);
-          tmem_wait_ld();
+        uint32_t w[32];
+        tmem_ld32(ts, s);
+        tmem_wait_ld();
+#pragma unroll
+        for (int h = 0; h < 2; h++) {   // 64 keys at a time; the next 32 columns are read meanwhile
+          tmem_ld32(ts + 64 * h + 32, s1);
           weights32(s, scale2, nref2, sum2, w);
+          tmem_wait_ld();
+          if (h == 0) tmem_ld32(ts + 64, s);
           weights32(s1, scale2, nref2, sum2, w + 16);
-          tmem_st32(ts + c0 / 2, w);   // over S columns that have been read
+          if (h == 0) tmem_wait_ld();
+          tmem_st32(ts + 32 * h, w);   // over S columns that have been read
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pfull[2 * h + t]);
         }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&pfull[t]);
       }
       if (n > 0 && ok) {
         ok = mbar_wait_limit(&odone[t], (n - 1) & 1, SPIN_LIMIT, c.status);
