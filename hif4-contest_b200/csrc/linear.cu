@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
       uint32_t d[16];
       if (steps > 0) {
         tmem_ld16(tmem_d + lanes + n, d);
-        tmem_wait_ld();
+        tmem_wait_ld(d);
       } else {
 #pragma unroll
         for (int k = 0; k < 16; k++) d[k] = 0u;

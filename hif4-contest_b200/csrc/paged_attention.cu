@@ -396,12 +396,15 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(const AttendArgs a) {
 //                   dims: an MN-major B operand, so nothing is transposed)
 //   warps 12-15     decode the packed K and V tiles to bf16 in shared memory,
 //                   two stages each, words one half step ahead in registers
-// While one tile's softmax runs, the tensor core works on the other tile.
-// S and P of a tile share columns (S0 S1 O0 O1 fill the 512 columns at dh
-// 128), so S of the next step waits for the second product of this one.  The
-// softmax reference moves as in attend_rows_kernel, only past 2^8; then the
-// row's O is rescaled in tensor memory by the softmax warp itself: the
-// product that reads it next waits for this step's weights anyway.
+// S0 S1 O0 O1 fill the 512 columns at dh 128 and the weights lie over their
+// scores, so the softmax goes by half steps of 64 keys: a tile's two halves
+// are two buffers, and while one is in the softmax the tensor core finishes
+// the other's second product and computes its next scores.  (With one buffer
+// of 128 keys a tile's softmax and products ran one after the other: 4820
+// cycles a step for the 2048 that each of the tensor core, the exponentials
+// and shared memory needs.)  The softmax reference moves as in
+// attend_rows_kernel, only past 2^8; then the row's O is rescaled in tensor
+// memory by the softmax warp, once the product before has finished.
 namespace tiles {
 
 using namespace tc;
@@ -493,7 +496,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t *kfull = reinterpret_cast<uint64_t *>(smem + C::BARS), *kempty = kfull + 2, *vfull = kempty + 2;
-  uint64_t *vempty = vfull + 2, *sfull = vempty + 2, *pfull = sfull + 2, *odone = pfull + 4;
+  uint64_t *vempty = vfull + 2, *sfull = vempty + 2, *pfull = sfull + 4, *odone = pfull + 4;
   uint64_t *drain = odone + 2;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 2);
   int *found = reinterpret_cast<int *>(tmem_slot + 1);          // sequence, tile
@@ -537,6 +540,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         mbar_init(&vfull[i], 4);
         mbar_init(&vempty[i], two);
         mbar_init(&sfull[i], 1);
+        mbar_init(&sfull[2 + i], 1);
         mbar_init(&pfull[i], 4);
         mbar_init(&pfull[2 + i], 4);
         mbar_init(&odone[i], 1);
@@ -648,41 +652,39 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
       const uint64_t dq = smem_desc(base + C::Q + t * C::TILE, 16u, 1024u, 2u);
       const uint64_t dk = smem_desc(base + C::K, 16u, 1024u, 2u), dv = smem_desc(base + C::V, C::PANEL, 1024u, 2u);
       const uint32_t d_s = tmem + t * 128, d_o = tmem + 256 + t * 128;
-#pragma unroll 1
-      for (int i = 0; i <= n; i++) {
-        if (i > 0) {   // O += P V of step i - 1, in two halves of 64 keys as the weights come
-          const int s = (i - 1) & 1;
-          const uint64_t v = dv + s * (C::TILE >> 4);
-          ok = mbar_wait_limit(&vfull[s], ((i - 1) >> 1) & 1, SPIN_LIMIT, c.status) &&
-               mbar_wait_limit(&pfull[t], s, SPIN_LIMIT, c.status);
-          if (!ok) break;
-          tc_fence_after();
+      // half step j: 64 keys, S and weights of it in half j & 1 of the tile's columns
+      auto qk = [&](int j) {
+        const int st = (j >> 1) & 1;
+        const uint64_t k = dk + st * (C::TILE >> 4) + (j & 1) * (64 * 128 >> 4);
+        ok = mbar_wait_limit(&kfull[st], (j >> 2) & 1, SPIN_LIMIT, c.status);
+        if (!ok) return;
+        tc_fence_after();
 #pragma unroll
-          for (int j = 0; j < KEYS / 32; j++)
-            mma_f16_ts(d_o, d_s + j * 8, v + j * (2048 >> 4), idesc_bf16(DH, 1), (i > 1 || j > 0) ? 1u : 0u);
-          ok = mbar_wait_limit(&pfull[2 + t], s, SPIN_LIMIT, c.status);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int j = KEYS / 32; j < KEYS / 16; j++)
-            mma_f16_ts(d_o, d_s + j * 8, v + j * (2048 >> 4), idesc_bf16(DH, 1), 1u);
-          mma_commit(&odone[t]);
-          mma_commit(&vempty[s]);
+        for (int x = 0; x < DH / 16; x++) {
+          const uint32_t off = ((x >> 2) * C::PANEL + (x & 3) * 32) >> 4;
+          mma_f16_ss(d_s + (j & 1) * 64, dq + off, k + off, idesc_bf16(64, 0), x > 0 ? 1u : 0u);
         }
-        if (i < n) {   // S of step i, over the weights of step i - 1
-          const int s = i & 1;
-          const uint64_t k = dk + s * (C::TILE >> 4);
-          ok = mbar_wait_limit(&kfull[s], (i >> 1) & 1, SPIN_LIMIT, c.status) &&
-               (i == 0 || mbar_wait_limit(&odone[t], (i - 1) & 1, SPIN_LIMIT, c.status));
-          if (!ok) break;
-          tc_fence_after();
+        mma_commit(&sfull[2 * t + (j & 1)]);
+        if (j & 1) mma_commit(&kempty[st]);
+      };
+      qk(0);
+      if (ok) qk(1);
+#pragma unroll 1
+      for (int j = 0; j < 2 * n && ok; j++) {
+        const int st = (j >> 1) & 1;
+        const uint64_t v = dv + st * (C::TILE >> 4) + (j & 1) * (64 * 128 >> 4);
+        ok = mbar_wait_limit(&vfull[st], (j >> 2) & 1, SPIN_LIMIT, c.status) &&
+             mbar_wait_limit(&pfull[2 * t + (j & 1)], (j >> 1) & 1, SPIN_LIMIT, c.status);
+        if (!ok) break;
+        tc_fence_after();
 #pragma unroll
-          for (int j = 0; j < DH / 16; j++) {
-            const uint32_t off = ((j >> 2) * C::PANEL + (j & 3) * 32) >> 4;
-            mma_f16_ss(d_s, dq + off, k + off, idesc_bf16(KEYS, 0), j > 0 ? 1u : 0u);
-          }
-          mma_commit(&sfull[t]);
-          mma_commit(&kempty[s]);
+        for (int x = 0; x < 4; x++)
+          mma_f16_ts(d_o, d_s + (j & 1) * 64 + x * 8, v + x * (2048 >> 4), idesc_bf16(DH, 1), (j > 0 || x > 0) ? 1u : 0u);
+        mma_commit(&odone[t]);
+        if (j & 1) mma_commit(&vempty[st]);
+        if (j + 2 < 2 * n) {   // the next S of these columns, once their weights have been read
+          ok = mbar_wait_limit(&odone[t], j & 1, SPIN_LIMIT, c.status);
+          if (ok) qk(j + 2);
         }
       }
       mma_commit(&drain[t]);   // every issued product has finished before tensor memory is released
@@ -704,92 +706,75 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
       float ref = -INFINITY;
       u64 sum2 = pk2(0.0f, 0.0f);
 #pragma unroll 1
-      for (int i = 0; i < n; i++) {
-        ok = mbar_wait_limit(&sfull[t], i & 1, SPIN_LIMIT, c.status);
+      for (int j = 0; j < 2 * n; j++) {
+        const int i = j >> 1, h = j & 1;
+        ok = mbar_wait_limit(&sfull[2 * t + h], i & 1, SPIN_LIMIT, c.status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        const int key0 = kt.key0(first + i, KEYS);
-        const uint32_t hid = *reinterpret_cast<const uint32_t *>(hidden + (i & 3) * 4);
-        const bool all = key0 + KEYS - 1 <= t_lo &&
-                         (a.window == 0 || key0 > t_hi - a.window || key0 + KEYS - 1 < a.sinks) && hid == 0;
         uint32_t s[32], s1[32];
-        // the row's largest score; where not all keys are visible, hidden columns are -inf from here on
-        float m = -INFINITY;
-        if (all) {
-#pragma unroll 1
-          for (int c0 = 0; c0 < KEYS; c0 += 64) {
-            tmem_ld32(ts + c0, s);
-            tmem_ld32(ts + c0 + 32, s1);
-            tmem_wait_ld();
-            float x[4] = {m, m, m, m};
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              x[0] = max3(x[0], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
-              x[1] = max3(x[1], __uint_as_float(s[j + 2]), __uint_as_float(s[j + 3]));
-              x[2] = max3(x[2], __uint_as_float(s1[j]), __uint_as_float(s1[j + 1]));
-              x[3] = max3(x[3], __uint_as_float(s1[j + 2]), __uint_as_float(s1[j + 3]));
-            }
-            m = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-          }
-        } else {
-          // visible columns: j <= hi and (j > lo or j < sk), 16-key blocks with a page
+        tmem_ld32(ts + 64 * h, s);
+        tmem_ld32(ts + 64 * h + 32, s1);
+        const int key0 = kt.key0(first + i, KEYS) + 64 * h;
+        const uint32_t hid = *reinterpret_cast<const uint16_t *>(hidden + (i & 3) * 4 + 2 * h);   // a bit for 16 keys: 0 1 8 9
+        const bool all = key0 + 63 <= t_lo && (a.window == 0 || key0 > t_hi - a.window || key0 + 63 < a.sinks) && hid == 0;
+        tmem_wait_ld(s);
+        tmem_loaded(s1);
+        if (!all) {
+          // visible columns: x <= hi and (x > lo or x < sk), 16-key blocks with a page
           const int hi = p - key0, lo = a.window ? p - a.window - key0 : -1, sk = a.sinks - key0;
-#pragma unroll 1
-          for (int c0 = 0; c0 < KEYS; c0 += 32) {
-            tmem_ld32(ts + c0, s);
-            tmem_wait_ld();
-            const uint32_t hb = hid >> (c0 / 4);
 #pragma unroll
-            for (int j = 0; j < 32; j++) {
-              const int col = c0 + j;
-              const bool see = col <= hi && (col > lo || col < sk) && !((hb >> (j / 16)) & 1u);
-              s[j] = see ? s[j] : 0xff800000u;
-              m = fmaxf(m, __uint_as_float(s[j]));
-            }
-            tmem_st32(ts + c0, s);
+          for (int x = 0; x < 32; x++) {
+            const bool see = x <= hi && (x > lo || x < sk) && !((hid >> (x / 16)) & 1u);
+            s[x] = see ? s[x] : 0xff800000u;
+            const bool see1 = x + 32 <= hi && (x + 32 > lo || x + 32 < sk) && !((hid >> (8 + x / 16)) & 1u);
+            s1[x] = see1 ? s1[x] : 0xff800000u;
           }
-          tmem_wait_st();
         }
-        m *= a.scale;
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int x = 0; x < 32; x += 4) {
+          m4[0] = max3(m4[0], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
+          m4[1] = max3(m4[1], __uint_as_float(s[x + 2]), __uint_as_float(s[x + 3]));
+          m4[2] = max3(m4[2], __uint_as_float(s1[x]), __uint_as_float(s1[x + 1]));
+          m4[3] = max3(m4[3], __uint_as_float(s1[x + 2]), __uint_as_float(s1[x + 3]));
+        }
+        const float m = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * a.scale;
         if (__any_sync(0xffffffffu, m > ref + kLazy)) {
           const float to_ref = fmaxf(m, ref);
           const float f = ref == -INFINITY ? 0.0f : ex2(ref - to_ref);
           ref = to_ref;
           sum2 = mul2(sum2, pk2(f, f));
-          if (i > 0) {
+          if (j > 0) {   // O as of the half step before
+            ok = mbar_wait_limit(&odone[t], (j - 1) & 1, SPIN_LIMIT, c.status);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll 1
-            for (int c0 = 0; c0 < DH; c0 += 32) {
-              tmem_ld32(to + c0, s);
-              tmem_wait_ld();
+            for (int c0 = 0; c0 < DH; c0 += 16) {
+              uint32_t x[16];
+              tmem_ld16(to + c0, x);
+              tmem_wait_ld(x);
 #pragma unroll
-              for (int j = 0; j < 32; j++) s[j] = __float_as_uint(__uint_as_float(s[j]) * f);
-              tmem_st32(to + c0, s);
+              for (int k = 0; k < 16; k++) x[k] = __float_as_uint(__uint_as_float(x[k]) * f);
+              tmem_st16(to + c0, x);
             }
           }
         }
         const float base = ref == -INFINITY ? 0.0f : ref;
         const u64 scale2 = pk2(a.scale, a.scale), nref2 = pk2(-base, -base);
         uint32_t w[32];
-        tmem_ld32(ts, s);
-        tmem_wait_ld();
-#pragma unroll
-        for (int h = 0; h < 2; h++) {   // 64 keys at a time; the next 32 columns are read meanwhile
-          tmem_ld32(ts + 64 * h + 32, s1);
-          weights32(s, scale2, nref2, sum2, w);
-          tmem_wait_ld();
-          if (h == 0) tmem_ld32(ts + 64, s);
-          weights32(s1, scale2, nref2, sum2, w + 16);
-          if (h == 0) tmem_wait_ld();
-          tmem_st32(ts + 32 * h, w);   // over S columns that have been read
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&pfull[2 * h + t]);
-        }
+        weights32(s, scale2, nref2, sum2, w);
+        weights32(s1, scale2, nref2, sum2, w + 16);
+        tmem_st32(ts + 64 * h, w);   // over S columns that have been read
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        // a barrier for each half: a warp may be done with the next one before another is with this one
+        if (lane == 0) mbar_arrive(&pfull[2 * t + h]);
       }
       if (n > 0 && ok) {
-        ok = mbar_wait_limit(&odone[t], (n - 1) & 1, SPIN_LIMIT, c.status);
+        ok = mbar_wait_limit(&drain[t], 0, SPIN_LIMIT, c.status);   // all products
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
@@ -807,7 +792,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         uint32_t o[32];
         if (n > 0) {
           tmem_ld32(to + c0, o);
-          tmem_wait_ld();
+          tmem_wait_ld(o);
         } else {
 #pragma unroll
           for (int j = 0; j < 32; j++) o[j] = 0u;
