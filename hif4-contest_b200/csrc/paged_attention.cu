@@ -394,8 +394,8 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(const AttendArgs a) {
 //   warps 8, 9      one lane each issues a tile's products (tcgen05.mma kind::f16):
 //                   S = Q K^T (K-major K) and O += P V (V as it lies, keys by
 //                   dims: an MN-major B operand, so nothing is transposed)
-//   warps 12-15     decode the packed K and V tiles to bf16 in shared memory,
-//                   two stages each, words one half step ahead in registers
+//   warps 12-19     decode the packed K and V tiles to bf16 in shared memory,
+//                   two stages each, the next tile's words in registers
 // S0 S1 O0 O1 fill the 512 columns at dh 128 and the weights lie over their
 // scores, so the softmax goes by half steps of 64 keys: a tile's two halves
 // are two buffers, and while one is in the softmax the tensor core finishes
@@ -409,7 +409,7 @@ namespace tiles {
 
 using namespace tc;
 
-constexpr int THREADS = 512, KEYS = 128, ROWS = 256;
+constexpr int THREADS = 640, KEYS = 128, ROWS = 256;
 
 template <int DH>
 struct Cfg {
@@ -417,56 +417,55 @@ struct Cfg {
   static constexpr int PANEL = 128 * 128;                   // 64 dims of it
   static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE;   // two Q tiles, two stages of K and of V
   static constexpr int BARS = 6 * TILE;
-  static constexpr int SMEM = BARS + 256 + 1024;
+  static constexpr int SMEM = BARS + 512 + 1024;
 };
 
-// keys a 16-byte code chunk of a warp lands on: lane -> (key of the run, chunk of 32 dims)
+// A warp's 16 keys of a K or V tile, packed in registers: lane -> (key of a
+// run of eight or sixteen, 16-byte chunk of 32 dims).
 template <int DH>
 struct Loader {
-  static constexpr int CPR = DH / 32;          // chunks per row; also steps per 32 keys
-  static constexpr int KPI = 32 / CPR;         // keys per step
-  uint4 w[CPR];
-  uint32_t m[CPR], have;                       // have: bit per step
+  static constexpr int CPR = DH / 32;          // chunks per row
+  static constexpr int KPI = 32 / CPR;         // keys per load
+  static constexpr int N = 16 / KPI;           // loads
+  uint4 w[N];
+  uint32_t m[N];
+  bool have[N];
 
-  // words of keys [key0 + 32 warp, + 32); pg: page ids of its two 16-key blocks (-1: none)
-  __device__ __forceinline__ void load(const CacheArgs &c, int which, int kh, int key_first, const int (&pg)[2],
-                                       int last, int lane) {
-    const int ch = lane >> 3;
-    have = 0;
+  static __device__ __forceinline__ int key(int lane) { return (lane & 7) + (CPR == 2 ? 8 * (lane >> 4) : 0); }
+  static __device__ __forceinline__ int chunk(int lane) { return CPR == 4 ? lane >> 3 : (lane >> 3) & 1; }
+
+  // keys first .. first + 15, all of page `page` (negative: none); behind `last` there are none
+  __device__ __forceinline__ void load(const CacheArgs &c, int which, int kh, int first, int page, int last, int lane) {
+    const int64_t row = ((int64_t)max(page, 0) * c.heads + kh) * c.page_size + (first & (c.page_size - 1)) + key(lane);
+    const uint4 *src = reinterpret_cast<const uint4 *>(c.codes[which] + row * (DH / 2)) + chunk(lane);
+    const uint32_t *meta = c.meta[which] + row * (DH / 64) + (CPR == 4 ? chunk(lane) >> 1 : 0);
 #pragma unroll
-    for (int it = 0; it < CPR; it++) {
-      const int k = it * KPI + (lane & 7) + (CPR == 2 ? 8 * (ch >> 1) : 0);
-      const int key = key_first + k, page = pg[(it * KPI) >> 4];
-      if (page >= 0 && key <= last) {
-        const int64_t row = ((int64_t)page * c.heads + kh) * c.page_size + (key & (c.page_size - 1));
-        const int cc = CPR == 4 ? ch : ch & 1;
-        w[it] = __ldg(reinterpret_cast<const uint4 *>(c.codes[which] + row * (DH / 2)) + cc);
-        m[it] = __ldg(c.meta[which] + row * (DH / 64) + (CPR == 4 ? cc >> 1 : 0));
-        have |= 1u << it;
-      }
+    for (int it = 0; it < N; it++) {
+      w[it] = __ldg(src + it * KPI * (DH / 32));
+      m[it] = __ldg(meta + it * KPI * (DH / 64));
+      have[it] = page >= 0 && first + it * KPI + key(lane) <= last;
     }
   }
   // decoded into a tile: panel of 64 dims, key rows of 128 bytes, 16-byte chunk q at q ^ (key & 7); inside a
   // chunk the dims stand as (0 2 4 6 1 3 5 7), as Q's do
   __device__ __forceinline__ void store(uint8_t *tile, int warp, int lane) const {
-    const int ch = lane >> 3, q0 = (ch & 1) * 4;   // first sub-block of the group = 16-byte chunk of the panel row
+    const int ch = chunk(lane), q0 = (ch & 1) * 4;   // first sub-block of the group = 16-byte chunk of the panel row
 #pragma unroll
-    for (int it = 0; it < CPR; it++) {
-      const int key = warp * 32 + it * KPI + (lane & 7) + (CPR == 2 ? 8 * (ch >> 1) : 0);
-      uint8_t *row = tile + (CPR == 4 ? (ch >> 1) * Cfg<DH>::PANEL : 0) + key * 128;
-      const bool ok = (have >> it) & 1u;
-      const uint32_t mm = ok ? m[it] : 0u, sf2 = hif4_sf2(mm);
+    for (int it = 0; it < N; it++) {
+      const int k = warp * 16 + it * KPI + key(lane);
+      uint8_t *row = tile + (CPR == 4 ? (ch >> 1) * Cfg<DH>::PANEL : 0) + k * 128;
+      const uint32_t mm = have[it] ? m[it] : 0u, sf2 = hif4_sf2(mm);
       const Hif4Levels l(mm, q0);
-      const uint4 c = ok ? w[it] : make_uint4(0, 0, 0, 0);   // code 0 decodes to 0
+      const uint4 c = have[it] ? w[it] : make_uint4(0, 0, 0, 0);   // code 0 decodes to 0
       uint32_t o[4];
       hif4_decode8_even_odd<0>(c.x, l, sf2, o);
-      *reinterpret_cast<uint4 *>(row + ((q0 ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4 *>(row + ((q0 ^ (k & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
       hif4_decode8_even_odd<1>(c.y, l, sf2, o);
-      *reinterpret_cast<uint4 *>(row + (((q0 + 1) ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4 *>(row + (((q0 + 1) ^ (k & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
       hif4_decode8_even_odd<2>(c.z, l, sf2, o);
-      *reinterpret_cast<uint4 *>(row + (((q0 + 2) ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4 *>(row + (((q0 + 2) ^ (k & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
       hif4_decode8_even_odd<3>(c.w, l, sf2, o);
-      *reinterpret_cast<uint4 *>(row + (((q0 + 3) ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4 *>(row + (((q0 + 3) ^ (k & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   }
 };
@@ -484,6 +483,20 @@ __device__ __forceinline__ void weights32(const uint32_t (&s)[32], u64 scale2, u
   }
 }
 
+// bits 0 .. n - 1 (none for n <= 0, all for n >= 64)
+__device__ __forceinline__ u64 below(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
+
+// Registers move from the warps that need few to the softmax: 256 x 144 +
+// 256 x 72 + 128 x 40 = 60416 of the launch's 640 x 96 = 61440.
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -497,10 +510,10 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t *kfull = reinterpret_cast<uint64_t *>(smem + C::BARS), *kempty = kfull + 2, *vfull = kempty + 2;
   uint64_t *vempty = vfull + 2, *sfull = vempty + 2, *pfull = sfull + 4, *odone = pfull + 4;
-  uint64_t *drain = odone + 2;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 2);
+  uint64_t *drain = odone + 2, *turn = drain + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(turn + 8);
   int *found = reinterpret_cast<int *>(tmem_slot + 1);          // sequence, tile
-  uint8_t *hidden = reinterpret_cast<uint8_t *>(found + 2);     // [4 steps][4 warps]: 16-key blocks without a page
+  uint8_t *hidden = reinterpret_cast<uint8_t *>(found + 3);     // [4 steps][8 blocks of 16 keys]: 1 without a page
   const CacheArgs &c = a.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kh = blockIdx.y, split = blockIdx.z;
@@ -535,9 +548,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
       found[0] = seq;
       found[1] = tile;
       for (int i = 0; i < 2; i++) {
-        mbar_init(&kfull[i], 4);
+        mbar_init(&kfull[i], 8);
         mbar_init(&kempty[i], two);
-        mbar_init(&vfull[i], 4);
+        mbar_init(&vfull[i], 8);
         mbar_init(&vempty[i], two);
         mbar_init(&sfull[i], 1);
         mbar_init(&sfull[2 + i], 1);
@@ -546,6 +559,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         mbar_init(&odone[i], 1);
         mbar_init(&drain[i], 1);
       }
+      for (int i = 0; i < 8; i++) mbar_init(&turn[i], 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
   }
@@ -601,38 +615,33 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
 
   if (warp >= 12) {
     // ---- decode
+    regs_down<72>();
     const int w = warp - 12;
     const int *pages = c.pages + seq * c.ld_pages;
     const int last = p_hi;
-    // half step u: K (even) or V (odd) of step u / 2; the next one's words are on their way meanwhile
+    // item u: K (even) or V (odd) of step u / 2; the next one's words are on their way meanwhile, and so is what
+    // the page table says of the step after
     Loader<DH> cur, next;
-    auto look = [&](int i, int (&pg)[2]) {   // page ids of this warp's 32 keys of step i
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int key = kt.key0(first + i, KEYS) + w * 32 + h * 16;
-        pg[h] = -1;
-        if (i < n && key <= last) {
-          const int p = __ldg(pages + (key >> c.page_shift));
-          if (p >= 0 && p < c.num_pages) pg[h] = p;
-          else if (lane == 0) atomicExch(c.status, HIF4X_BAD_PAGE);
-        }
-      }
+    auto key_of = [&](int i) { return kt.key0(first + i, KEYS) + w * 16; };
+    auto look = [&](int i) { return i < n && key_of(i) <= last ? __ldg(pages + (key_of(i) >> c.page_shift)) : -1; };
+    auto check = [&](int i, int page) {   // an id of no page: -1, and reported where the keys exist
+      if (page >= 0 && page < c.num_pages) return page;
+      if (lane == 0 && i < n && key_of(i) <= last) atomicExch(c.status, HIF4X_BAD_PAGE);
+      return -1;
     };
-    int now[2], nxt[2];   // of the step being decoded, of the step after it
-    look(0, now);
-    look(1, nxt);
-    if (n > 0) cur.load(c, 0, kh, kt.key0(first, KEYS) + w * 32, now, last, lane);
+    int now = look(0), nxt = look(1);   // of the step being decoded, of the one after it
+    now = check(0, now);
+    if (n > 0) cur.load(c, 0, kh, key_of(0), now, last, lane);
 #pragma unroll 1
     for (int u = 0; u < 2 * n; u++) {
       const int i = u >> 1, v = u & 1, s = i & 1;
       if (v == 0) {
-        next.load(c, 1, kh, kt.key0(first + i, KEYS) + w * 32, now, last, lane);
-        if (lane == 0) hidden[(i & 3) * 4 + w] = (uint8_t)((now[0] < 0 ? 1 : 0) | (now[1] < 0 ? 2 : 0));
+        next.load(c, 1, kh, key_of(i), now, last, lane);
+        if (lane == 0) hidden[(i & 3) * 8 + w] = now < 0 ? 1 : 0;
       } else if (i + 1 < n) {
-        next.load(c, 0, kh, kt.key0(first + i + 1, KEYS) + w * 32, nxt, last, lane);
-        now[0] = nxt[0];
-        now[1] = nxt[1];
-        look(i + 2, nxt);
+        now = check(i + 1, nxt);
+        next.load(c, 0, kh, key_of(i + 1), now, last, lane);
+        nxt = look(i + 2);
       }
       if (i >= 2) ok = mbar_wait_limit((v ? vempty : kempty) + s, ((i >> 1) - 1) & 1, SPIN_LIMIT, c.status);
       ok = __all_sync(0xffffffffu, ok);
@@ -643,8 +652,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
       if (lane == 0) mbar_arrive((v ? vfull : kfull) + s);
       cur = next;
     }
-  } else if (warp == 8 || warp == 9) {
+  } else if (warp >= 8) {
     // ---- both products of tile warp - 8
+    regs_down<40>();
     const int t = warp - 8;
     if (t < tiles_here && n > 0 && elect_one()) {
       const uint32_t base = smem_u32(smem);
@@ -691,8 +701,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
       mbar_wait_limit(&drain[t], 0, SPIN_LIMIT, c.status);
     }
     __syncwarp();
-  } else if (warp < 8) {
+  } else {
     // ---- softmax: this thread's row
+    regs_up<144>();
     const int t = warp >> 2;
     const int r = t * 128 + (warp & 3) * 32 + lane;
     const int64_t rr = r0 + r;
@@ -716,28 +727,30 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         tmem_ld32(ts + 64 * h, s);
         tmem_ld32(ts + 64 * h + 32, s1);
         const int key0 = kt.key0(first + i, KEYS) + 64 * h;
-        const uint32_t hid = *reinterpret_cast<const uint16_t *>(hidden + (i & 3) * 4 + 2 * h);   // a bit for 16 keys: 0 1 8 9
+        const uint32_t hid = *reinterpret_cast<const uint32_t *>(hidden + (i & 3) * 8 + 4 * h);   // a byte for 16 keys
         const bool all = key0 + 63 <= t_lo && (a.window == 0 || key0 > t_hi - a.window || key0 + 63 < a.sinks) && hid == 0;
         tmem_wait_ld(s);
         tmem_loaded(s1);
         if (!all) {
-          // visible columns: x <= hi and (x > lo or x < sk), 16-key blocks with a page
+          // visible columns: y <= hi and (y > lo or y < sk), 16-key blocks with a page
           const int hi = p - key0, lo = a.window ? p - a.window - key0 : -1, sk = a.sinks - key0;
+          const u64 see = below(hi + 1) & (~below(lo + 1) | below(sk)) &
+                          ~((hid & 1u ? 0xffffull : 0ull) | (hid & 0x100u ? 0xffffull << 16 : 0ull) |
+                            (hid & 0x10000u ? 0xffffull << 32 : 0ull) | (hid & 0x1000000u ? 0xffffull << 48 : 0ull));
+          const uint32_t see0 = (uint32_t)see, see1 = (uint32_t)(see >> 32);
 #pragma unroll
-          for (int x = 0; x < 32; x++) {
-            const bool see = x <= hi && (x > lo || x < sk) && !((hid >> (x / 16)) & 1u);
-            s[x] = see ? s[x] : 0xff800000u;
-            const bool see1 = x + 32 <= hi && (x + 32 > lo || x + 32 < sk) && !((hid >> (8 + x / 16)) & 1u);
-            s1[x] = see1 ? s1[x] : 0xff800000u;
+          for (int y = 0; y < 32; y++) {
+            if (!(see0 & (1u << y))) s[y] = 0xff800000u;
+            if (!(see1 & (1u << y))) s1[y] = 0xff800000u;
           }
         }
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int x = 0; x < 32; x += 4) {
-          m4[0] = max3(m4[0], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
-          m4[1] = max3(m4[1], __uint_as_float(s[x + 2]), __uint_as_float(s[x + 3]));
-          m4[2] = max3(m4[2], __uint_as_float(s1[x]), __uint_as_float(s1[x + 1]));
-          m4[3] = max3(m4[3], __uint_as_float(s1[x + 2]), __uint_as_float(s1[x + 3]));
+        for (int y = 0; y < 32; y += 4) {
+          m4[0] = max3(m4[0], __uint_as_float(s[y]), __uint_as_float(s[y + 1]));
+          m4[1] = max3(m4[1], __uint_as_float(s[y + 2]), __uint_as_float(s[y + 3]));
+          m4[2] = max3(m4[2], __uint_as_float(s1[y]), __uint_as_float(s1[y + 1]));
+          m4[3] = max3(m4[3], __uint_as_float(s1[y + 2]), __uint_as_float(s1[y + 3]));
         }
         const float m = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * a.scale;
         if (__any_sync(0xffffffffu, m > ref + kLazy)) {
@@ -752,21 +765,31 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
             tc_fence_after();
 #pragma unroll 1
             for (int c0 = 0; c0 < DH; c0 += 16) {
-              uint32_t x[16];
-              tmem_ld16(to + c0, x);
-              tmem_wait_ld(x);
+              uint32_t y[16];
+              tmem_ld16(to + c0, y);
+              tmem_wait_ld(y);
 #pragma unroll
-              for (int k = 0; k < 16; k++) x[k] = __float_as_uint(__uint_as_float(x[k]) * f);
-              tmem_st16(to + c0, x);
+              for (int k = 0; k < 16; k++) y[k] = __float_as_uint(__uint_as_float(y[k]) * f);
+              tmem_st16(to + c0, y);
             }
           }
         }
         const float base = ref == -INFINITY ? 0.0f : ref;
         const u64 scale2 = pk2(a.scale, a.scale), nref2 = pk2(-base, -base);
+        // the two warps of a scheduler, one of each tile, take turns at the exponentials: at the same time they
+        // would halve each other's rate and then leave both tiles to the tensor core at once
+        if (tiles_here == 2 && (t == 1 || j > 0)) {
+          ok = mbar_wait_limit(&turn[warp ^ 4], (j - 1 + t) & 1, SPIN_LIMIT, c.status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tmem_loaded(s);   // the arithmetic stays behind the wait
+          tmem_loaded(s1);
+        }
         uint32_t w[32];
         weights32(s, scale2, nref2, sum2, w);
         weights32(s1, scale2, nref2, sum2, w + 16);
         tmem_st32(ts + 64 * h, w);   // over S columns that have been read
+        if (lane == 0) mbar_arrive(&turn[warp]);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
