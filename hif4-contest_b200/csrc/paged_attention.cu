@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         next.load(c, 0, kh, key_of(i + 1), now, last, lane);
         nxt = look(i + 2);
       }
-      if (i >= 2) ok = mbar_wait_limit((v ? vempty : kempty) + s, ((i >> 1) - 1) & 1, SPIN_LIMIT, c.status);
+      if (i >= 2) ok = mbar_wait_sleep((v ? vempty : kempty) + s, ((i >> 1) - 1) & 1, c.status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       cur.store(smem + (v ? C::V : C::K) + s * C::TILE, w, lane);
@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
       auto qk = [&](int j) {
         const int st = (j >> 1) & 1;
         const uint64_t k = dk + st * (C::TILE >> 4) + (j & 1) * (64 * 128 >> 4);
-        ok = mbar_wait_limit(&kfull[st], (j >> 2) & 1, SPIN_LIMIT, c.status);
+        ok = mbar_wait_sleep(&kfull[st], (j >> 2) & 1, c.status);
         if (!ok) return;
         tc_fence_after();
 #pragma unroll
@@ -683,8 +683,8 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
       for (int j = 0; j < 2 * n && ok; j++) {
         const int st = (j >> 1) & 1;
         const uint64_t v = dv + st * (C::TILE >> 4) + (j & 1) * (64 * 128 >> 4);
-        ok = mbar_wait_limit(&vfull[st], (j >> 2) & 1, SPIN_LIMIT, c.status) &&
-             mbar_wait_limit(&pfull[2 * t + (j & 1)], (j >> 1) & 1, SPIN_LIMIT, c.status);
+        ok = mbar_wait_sleep(&vfull[st], (j >> 2) & 1, c.status) &&
+             mbar_wait_sleep(&pfull[2 * t + (j & 1)], (j >> 1) & 1, c.status);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
@@ -693,12 +693,12 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         mma_commit(&odone[t]);
         if (j & 1) mma_commit(&vempty[st]);
         if (j + 2 < 2 * n) {   // the next S of these columns, once their weights have been read
-          ok = mbar_wait_limit(&odone[t], j & 1, SPIN_LIMIT, c.status);
+          ok = mbar_wait_sleep(&odone[t], j & 1, c.status);
           if (ok) qk(j + 2);
         }
       }
       mma_commit(&drain[t]);   // every issued product has finished before tensor memory is released
-      mbar_wait_limit(&drain[t], 0, SPIN_LIMIT, c.status);
+      mbar_wait_sleep(&drain[t], 0, c.status);
     }
     __syncwarp();
   } else {
@@ -719,7 +719,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
 #pragma unroll 1
       for (int j = 0; j < 2 * n; j++) {
         const int i = j >> 1, h = j & 1;
-        ok = mbar_wait_limit(&sfull[2 * t + h], i & 1, SPIN_LIMIT, c.status);
+        ok = mbar_wait_sleep(&sfull[2 * t + h], i & 1, c.status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
@@ -759,7 +759,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
           ref = to_ref;
           sum2 = mul2(sum2, pk2(f, f));
           if (j > 0) {   // O as of the half step before
-            ok = mbar_wait_limit(&odone[t], (j - 1) & 1, SPIN_LIMIT, c.status);
+            ok = mbar_wait_sleep(&odone[t], (j - 1) & 1, c.status);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
@@ -779,7 +779,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         // the two warps of a scheduler, one of each tile, take turns at the exponentials: at the same time they
         // would halve each other's rate and then leave both tiles to the tensor core at once
         if (tiles_here == 2 && (t == 1 || j > 0)) {
-          ok = mbar_wait_limit(&turn[warp ^ 4], (j - 1 + t) & 1, SPIN_LIMIT, c.status);
+          ok = mbar_wait_sleep(&turn[warp ^ 4], (j - 1 + t) & 1, c.status);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tmem_loaded(s);   // the arithmetic stays behind the wait
@@ -797,7 +797,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         if (lane == 0) mbar_arrive(&pfull[2 * t + h]);
       }
       if (n > 0 && ok) {
-        ok = mbar_wait_limit(&drain[t], 0, SPIN_LIMIT, c.status);   // all products
+        ok = mbar_wait_sleep(&drain[t], 0, c.status);   // all products
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }

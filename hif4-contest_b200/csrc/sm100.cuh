@@ -52,6 +52,24 @@ __device__ __forceinline__ bool mbar_wait_limit(uint64_t *bar, uint32_t parity, 
   return false;
 }
 
+// The same with a hint that the thread may sleep up to a microsecond a poll:
+// warps of other roles on the scheduler then lose fewer issue slots to polling.
+__device__ __forceinline__ bool mbar_wait_sleep(uint64_t *bar, uint32_t parity, int *status) {
+  for (long long i = 0; i < SPIN_LIMIT; i++) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(1000)
+        : "memory");
+    if (ok) return true;
+  }
+  atomicExch(status, HIF4X_TIMEOUT);
+  return false;
+}
+
 // One lane of a converged warp.  The compiler knows that the branch has a
 // single thread, so what the tensor-core instructions take from uniform
 // registers is computed there (a test of the lane's number costs moves for
