@@ -911,33 +911,38 @@ struct AttendPlan {
 // the lengths: where max_new allows for more than 16 rows both kernels run and
 // each passes over the other's sequences, except that a single sequence is the
 // tiles kernel's alone.
-static int attend_plan(const hif4x_kv_cache *kv, const hif4x_kv_batch *b, int q_heads, int64_t rows, int window,
-                       int sinks, int max_new, AttendPlan *p) {
+struct AttendSizes {
+  int page_size, kv_heads, head_dim, sequences, max_pages, q_heads;
+  int64_t rows;
+  int window, sinks, max_new;
+};
+
+static int attend_plan(const AttendSizes &z, AttendPlan *p) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return HIF4X_ERR_LAUNCH;
   const int sms = tc::device_sms(dev);
   if (sms <= 0) return HIF4X_ERR_LAUNCH;
-  const int group = q_heads / kv->kv_heads;
-  const int64_t B = b->sequences, H = kv->kv_heads;
-  int64_t keys = (int64_t)b->max_pages * kv->page_size;
-  if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + max_new + sinks + 32);
-  p->tiles = (int64_t)max_new * group > 16;
+  const int group = z.q_heads / z.kv_heads;
+  const int64_t B = z.sequences, H = z.kv_heads;
+  int64_t keys = (int64_t)z.max_pages * z.page_size;
+  if (z.window > 0) keys = std::min<int64_t>(keys, (int64_t)z.window + z.max_new + z.sinks + 32);
+  p->tiles = (int64_t)z.max_new * group > 16;
   p->rows = !p->tiles || B > 1;
   p->most_rows = !p->tiles ? INT32_MAX : B > 1 ? 16 : 0;
   p->grid_tiles = 0;
   if (p->tiles) {
-    const int64_t n = rows * group / tiles::ROWS + B;
+    const int64_t n = z.rows * group / tiles::ROWS + B;
     if (n > INT32_MAX) return HIF4X_ERR_UNSUPPORTED;
     p->grid_tiles = (int)n;
     // shares of the keys: as many as fill the SMs once, four steps or more to each
-    const int64_t busy = std::max<int64_t>(1, rows * group / tiles::ROWS) * H;
+    const int64_t busy = std::max<int64_t>(1, z.rows * group / tiles::ROWS) * H;
     p->splits = (int)std::max<int64_t>(
-        1, std::min<int64_t>({sms / busy, keys / (4 * tiles::KEYS), (int64_t(1) << 26) / (rows * q_heads * kv->head_dim), 64}));
+        1, std::min<int64_t>({sms / busy, keys / (4 * tiles::KEYS), (int64_t(1) << 26) / (z.rows * z.q_heads * z.head_dim), 64}));
   } else {
-    p->splits = attend_splits(sms, B * H, keys, rows * q_heads * kv->head_dim);
+    p->splits = attend_splits(sms, B * H, keys, z.rows * z.q_heads * z.head_dim);
   }
-  p->part_floats = p->splits > 1 ? (int64_t)p->splits * rows * q_heads * kv->head_dim : 0;
-  p->work_bytes = p->splits > 1 ? p->part_floats * 4 + (int64_t)p->splits * rows * q_heads * 8 : 0;
+  p->part_floats = p->splits > 1 ? (int64_t)p->splits * z.rows * z.q_heads * z.head_dim : 0;
+  p->work_bytes = p->splits > 1 ? p->part_floats * 4 + (int64_t)p->splits * z.rows * z.q_heads * 8 : 0;
   return HIF4X_OK;
 }
 
@@ -960,30 +965,28 @@ static int launch_tiles(AttendArgs a, int dev, const AttendPlan &p, cudaStream_t
   return HIF4X_OK;
 }
 
-static int attend_check(const hif4x_kv_cache *kv, const hif4x_kv_batch *b, int q_heads, int64_t rows, int window,
-                        int sinks, int max_new, CacheArgs *c) {
-  const int st = cache_args(kv, b, rows, c);
-  if (st != HIF4X_OK) return st;
-  if (q_heads < kv->kv_heads || q_heads % kv->kv_heads || window < 0 || sinks < 0 || max_new < 1 ||
-      window > (1 << 30) || sinks > (1 << 30) || rows * q_heads > INT32_MAX)
-    return HIF4X_ERR_ARG;
-  return HIF4X_OK;
+static bool attend_sizes_ok(const AttendSizes &z) {
+  return z.kv_heads >= 1 && z.q_heads >= z.kv_heads && z.q_heads % z.kv_heads == 0 && z.window >= 0 && z.sinks >= 0 &&
+         z.max_new >= 1 && z.window <= (1 << 30) && z.sinks <= (1 << 30) && z.rows >= 0 &&
+         z.rows * z.q_heads <= INT32_MAX && z.sequences >= 1 && z.max_pages >= 1 && z.page_size >= 1 &&
+         (z.head_dim == 64 || z.head_dim == 128);
 }
 
 }  // namespace hif4x
 
 using namespace hif4x;
 
-extern "C" int hif4x_paged_attention_work(const hif4x_kv_cache *kv, const hif4x_kv_batch *batch, int q_heads,
-                                          int64_t rows, int window, int sinks, int max_new, int64_t *bytes) {
-  if (!bytes) return HIF4X_ERR_ARG;
-  CacheArgs c{};
-  const int st = attend_check(kv, batch, q_heads, rows, window, sinks, max_new, &c);
-  if (st != HIF4X_OK) return st;
+extern "C" int hif4x_paged_attention_work(int page_size, int kv_heads, int head_dim, int sequences, int max_pages,
+                                          int q_heads, int64_t rows, int window, int sinks, int max_new,
+                                          int64_t *bytes) {
+  const AttendSizes z{page_size, kv_heads, head_dim, sequences, max_pages, q_heads, rows, window, sinks, max_new};
+  if (!bytes || !attend_sizes_ok(z)) return HIF4X_ERR_ARG;
+  *bytes = 0;
+  if (rows == 0) return HIF4X_OK;
   AttendPlan p{};
-  const int st2 = attend_plan(kv, batch, q_heads, rows, window, sinks, max_new, &p);
+  const int st = attend_plan(z, &p);
   *bytes = p.work_bytes;
-  return st2;
+  return st;
 }
 
 extern "C" int hif4x_paged_attention(const hif4x_kv_cache *kv, const hif4x_kv_batch *batch, const void *q,
@@ -991,15 +994,18 @@ extern "C" int hif4x_paged_attention(const hif4x_kv_cache *kv, const hif4x_kv_ba
                                      int window, int sinks, int max_new, void *out, int64_t o_ld_row,
                                      int64_t o_ld_head, void *work, int64_t work_bytes, void *stream) {
   AttendArgs a{};
-  int st = attend_check(kv, batch, q_heads, rows, window, sinks, max_new, &a.c);
+  int st = cache_args(kv, batch, rows, &a.c);
   if (st != HIF4X_OK) return st;
+  const AttendSizes z{kv->page_size, kv->kv_heads, kv->head_dim, batch->sequences, batch->max_pages, q_heads,
+                      rows, window, sinks, max_new};
+  if (!attend_sizes_ok(z)) return HIF4X_ERR_ARG;
   if (rows == 0) return HIF4X_OK;
   if (!q || !out || q == out) return HIF4X_ERR_ARG;
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) || q_ld_row % 8 || q_ld_head % 8 ||
       o_ld_row % 8 || o_ld_head % 8)
     return HIF4X_ERR_ARG;
   AttendPlan p{};
-  st = attend_plan(kv, batch, q_heads, rows, window, sinks, max_new, &p);
+  st = attend_plan(z, &p);
   if (st != HIF4X_OK) return st;
   if (p.work_bytes > 0 && (!work || work_bytes < p.work_bytes || (reinterpret_cast<uintptr_t>(work) & 15u)))
     return HIF4X_ERR_ARG;

@@ -117,8 +117,7 @@ SIGNATURES: dict[str, list] = {
     "hif4x_kv_append": [ctypes.POINTER(KVCacheDesc), ctypes.POINTER(KVBatchDesc), vp, i64, i64, vp, i64, i64, i32,
                         i64, vp],
     "hif4x_kv_read": [ctypes.POINTER(KVCacheDesc), ctypes.POINTER(KVBatchDesc), i64, vp, vp, i32, vp],
-    "hif4x_paged_attention_work": [ctypes.POINTER(KVCacheDesc), ctypes.POINTER(KVBatchDesc), i32, i64, i32, i32, i32,
-                                   ctypes.POINTER(i64)],
+    "hif4x_paged_attention_work": [i32, i32, i32, i32, i32, i32, i64, i32, i32, i32, ctypes.POINTER(i64)],
     "hif4x_paged_attention": [ctypes.POINTER(KVCacheDesc), ctypes.POINTER(KVBatchDesc), vp, i64, i64, i32, i64, f32,
                               i32, i32, i32, vp, i64, i64, vp, i64, vp],
 }
@@ -152,8 +151,14 @@ def lib():
     return _LIB
 
 
+_FN: dict = {}   # entry points that have been called
+
+
 def call(name: str, *args) -> int:
-    st = getattr(lib(), name)(*args)
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(lib(), name)
+    st = fn(*args)
     if st < 0:
         raise Hif4xError(name, st)
     return st

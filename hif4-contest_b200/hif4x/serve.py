@@ -12,8 +12,8 @@ a CUDA graph.  linalg.check_device_status reports what a kernel found wrong
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -23,12 +23,22 @@ GROUP = 64
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 
-def _on(dev: torch.device):
-    """The device's context, where it is not the current one."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _call(dev: torch.device, name: str, *args) -> None:
+    """An entry point with the device's current stream behind its arguments, the device being the current one."""
+    index = dev.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch.cuda.current_device():
+        L.call(name, *args, stream)
+    else:
+        with torch.cuda.device(index):
+            L.call(name, *args, stream)
 
 
 def _cuda(t: torch.Tensor, name: str, dtypes, dim: int, dev: torch.device | None = None):
+    """The tensor has one of the dtypes and `dim` dimensions and is on `dev` (None: on any GPU)."""
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == dim and (
+            t.device == dev if dev is not None else t.is_cuda):
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
     if t.dtype not in dtypes:
@@ -37,8 +47,7 @@ def _cuda(t: torch.Tensor, name: str, dtypes, dim: int, dev: torch.device | None
         raise ValueError(f"{name} has {t.dim()} dimensions: {dim} wanted")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if dev is not None and t.device != dev:
-        raise ValueError(f"{name} is on {t.device}, the first tensor on {dev}")
+    raise ValueError(f"{name} is on {t.device}, the first tensor on {dev}")
 
 
 def _row_stride(t: torch.Tensor, name: str, aligned: bool) -> int:
@@ -117,10 +126,9 @@ def linear(x: torch.Tensor, meta: torch.Tensor, codes: torch.Tensor, bias: torch
             raise ValueError("out overlaps residual without being it")
     if T == 0:
         return out
-    with _on(dev):
-        L.call("hif4x_linear_packed", x.data_ptr(), ldx, meta.data_ptr(), codes.data_ptr(), T, N, C,
-               None if bias is None else bias.data_ptr(), bias_dtype, ACTIVATIONS[activation],
-               None if residual is None else residual.data_ptr(), ldr, out.data_ptr(), ldy, L.stream(dev))
+    _call(dev, "hif4x_linear_packed", x.data_ptr(), ldx, meta.data_ptr(), codes.data_ptr(), T, N, C,
+          None if bias is None else bias.data_ptr(), bias_dtype, ACTIVATIONS[activation],
+          None if residual is None else residual.data_ptr(), ldr, out.data_ptr(), ldy)
     return out
 
 
@@ -212,10 +220,8 @@ def kv_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, cu_new: torch.Te
     batch = cache._batch(cu_new, kv_len, pages)
     if k.shape[0] == 0:
         return
-    with _on(cache.device):
-        L.call("hif4x_kv_append", ctypes.byref(cache._desc), ctypes.byref(batch), k.data_ptr(), k.stride(0),
-               k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), L.dtype_code(k.dtype), k.shape[0],
-               L.stream(cache.device))
+    _call(cache.device, "hif4x_kv_append", ctypes.byref(cache._desc), ctypes.byref(batch), k.data_ptr(), k.stride(0),
+          k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), L.dtype_code(k.dtype), k.shape[0])
 
 
 def kv_read(cache: PagedKV, cu_new: torch.Tensor, kv_len: torch.Tensor, pages: torch.Tensor, rows: int,
@@ -239,10 +245,18 @@ def kv_read(cache: PagedKV, cu_new: torch.Tensor, kv_len: torch.Tensor, pages: t
         if rows and (k.data_ptr() % 16 or v.data_ptr() % 16 or _overlap(k, v)):
             raise ValueError("out must be two 16-byte aligned tensors apart")
     if rows:
-        with _on(cache.device):
-            L.call("hif4x_kv_read", ctypes.byref(cache._desc), ctypes.byref(batch), rows, k.data_ptr(), v.data_ptr(),
-                   L.dtype_code(k.dtype), L.stream(cache.device))
+        _call(cache.device, "hif4x_kv_read", ctypes.byref(cache._desc), ctypes.byref(batch), rows, k.data_ptr(),
+              v.data_ptr(), L.dtype_code(k.dtype))
     return k, v
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_work(dev: torch.device, *sizes: int) -> int:
+    """Bytes of workspace of an attention call of these sizes."""
+    need = L.i64()
+    with torch.cuda.device(dev):
+        L.call("hif4x_paged_attention_work", *sizes, ctypes.byref(need))
+    return need.value
 
 
 def paged_attention(q: torch.Tensor, cache: PagedKV, cu_new: torch.Tensor, kv_len: torch.Tensor, pages: torch.Tensor,
@@ -281,12 +295,10 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, cu_new: torch.Tensor, kv_le
     if rows == 0:
         return out
     most = min(rows, max_new) if max_new is not None else rows
-    need = L.i64()
-    desc, bdesc = ctypes.byref(cache._desc), ctypes.byref(batch)
-    with _on(cache.device):
-        L.call("hif4x_paged_attention_work", desc, bdesc, heads, rows, window, sinks, most, ctypes.byref(need))
-        work = torch.empty(need.value, dtype=torch.uint8, device=cache.device) if need.value else None
-        L.call("hif4x_paged_attention", desc, bdesc, q.data_ptr(), qr, qh, heads, rows,
-               dh ** -0.5 if scale is None else float(scale), window, sinks, most, out.data_ptr(), orow, ohead,
-               None if work is None else work.data_ptr(), need.value, L.stream(cache.device))
+    need = _attention_work(cache.device, cache.page_size, cache.kv_heads, dh, batch.sequences, batch.max_pages, heads,
+                           rows, window, sinks, most)
+    work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+    _call(cache.device, "hif4x_paged_attention", ctypes.byref(cache._desc), ctypes.byref(batch), q.data_ptr(), qr, qh,
+          heads, rows, dh ** -0.5 if scale is None else float(scale), window, sinks, most, out.data_ptr(), orow, ohead,
+          None if work is None else work.data_ptr(), need)
     return out

@@ -441,10 +441,11 @@ int hif4x_kv_read(const hif4x_kv_cache *kv, const hif4x_kv_batch *batch, int64_t
  * q_heads x head_dim bf16, strides in elements, multiples of 8, 16-byte
  * aligned; rows of no sequence are left as they were.  max_new: about how
  * many new rows a sequence has at most (it chooses the kernel; the result
- * holds for any).  work: hif4x_paged_attention_work bytes, 16-byte aligned
- * (NULL where that is 0), used until the call's kernels have run. */
-int hif4x_paged_attention_work(const hif4x_kv_cache *kv, const hif4x_kv_batch *batch, int q_heads, int64_t rows,
-                               int window, int sinks, int max_new, int64_t *bytes);
+ * holds for any).  work: hif4x_paged_attention_work bytes (they depend on the
+ * sizes and the current device alone), 16-byte aligned (NULL where that is
+ * 0), used until the call's kernels have run. */
+int hif4x_paged_attention_work(int page_size, int kv_heads, int head_dim, int sequences, int max_pages, int q_heads,
+                               int64_t rows, int window, int sinks, int max_new, int64_t *bytes);
 int hif4x_paged_attention(const hif4x_kv_cache *kv, const hif4x_kv_batch *batch, const void *q, int64_t q_ld_row,
                           int64_t q_ld_head, int q_heads, int64_t rows, float scale, int window, int sinks,
                           int max_new, void *out, int64_t o_ld_row, int64_t o_ld_head, void *work,

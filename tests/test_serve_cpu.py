@@ -41,10 +41,8 @@ def batch(**kw):
 
 def calls(kv, b, rows=2):
     lib, r = L.lib(), ctypes.byref
-    need = L.i64()
     yield lib.hif4x_kv_append(r(kv), r(b), P, 128, 64, P, 128, 64, L.DT_BF16, rows, None)
     yield lib.hif4x_kv_read(r(kv), r(b), rows, P, P, L.DT_BF16, None)
-    yield lib.hif4x_paged_attention_work(r(kv), r(b), 4, rows, 0, 0, 1, r(need))
     yield lib.hif4x_paged_attention(r(kv), r(b), P, 256, 64, 4, rows, 0.1, 0, 0, 1, P, 256, 64, None, 0, None)
 
 
@@ -58,6 +56,15 @@ def test_cache_and_batch_refusals():
                dict(ld_pages=2)):
         assert set(calls(cache(), batch(**kw))) == {L.ERR_ARG}, kw
     assert set(calls(cache(), batch(), rows=-1)) == {L.ERR_ARG}
+
+
+def test_attention_refusals():
+    lib, r, need = L.lib(), ctypes.byref, L.i64()
+    ok = dict(page=16, kvh=2, dh=64, B=2, most=3, qh=4, rows=2, window=0, sinks=0, max_new=1)
+    for kw in (dict(kvh=0), dict(dh=80), dict(B=0), dict(most=0), dict(qh=3), dict(qh=1), dict(rows=-1), dict(window=-1),
+               dict(sinks=-1), dict(window=2 ** 30 + 1), dict(sinks=2 ** 30 + 1), dict(max_new=0), dict(rows=2 ** 30)):
+        assert lib.hif4x_paged_attention_work(*{**ok, **kw}.values(), r(need)) == L.ERR_ARG, kw
+    assert lib.hif4x_paged_attention_work(*{**ok, "rows": 0}.values(), r(need)) == L.OK and need.value == 0
 
 
 def test_python_refuses_host_tensors():
