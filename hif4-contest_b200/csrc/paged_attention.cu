@@ -49,6 +49,7 @@ struct AttendArgs {
   float2 *part_ml;
 };
 
+constexpr int64_t MOST_SPLITS = 64;   // shares of a row's keys (attend_join_kernel: four warps, a lane for each of 16)
 constexpr float kLazy = 8.0f;    // log2 a row's scores may pass its reference by
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -100,40 +101,56 @@ struct KeyTiles {
   __device__ __forceinline__ int key0(int i, int tile) const { return (i < n_sink ? i : i - n_sink + first) * tile; }
 };
 
-// One 16-key tile's packed words in registers.
+// One 16-key tile's packed words in registers, and where this lane's lie
+// within the 16 rows of a tile.
 template <int DH>
 struct TileRegs {
   uint32_t k[2][DH / 32], km[2], v[4][DH / 64], vm[4];
-  __device__ __forceinline__ void load(const CacheArgs &c, int64_t row, int lane) {
+  const uint8_t *kc, *vc;
+  const uint32_t *kp, *vp;
+
+  __device__ __forceinline__ TileRegs(const CacheArgs &c, int lane) {
     const int n = lane >> 2, q = lane & 3;
-    constexpr int NB = DH / 64;
+    kc = c.codes[0] + n * (DH / 2) + q * (DH / 8);
+    kp = c.meta[0] + n * (DH / 64) + (DH == 128 ? q >> 1 : 0);
+    vc = c.codes[1] + 2 * q * (DH / 2) + n * (DH / 16);
+    vp = c.meta[1] + 2 * q * (DH / 64) + (DH == 128 ? n >> 2 : 0);
+  }
+  // rows n8 and n8 + 8 of the tile, this thread's quarter of the dims
+  __device__ __forceinline__ void load_k(int64_t row) {
+    const uint8_t *src = kc + row * (DH / 2);
+    const uint32_t *meta = kp + row * (DH / 64);
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      const int64_t r = row + n + 8 * u;
       if (DH == 128) {
-        const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(c.codes[0] + r * (DH / 2)) + q);
+        const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(src + u * 8 * (DH / 2)));
         k[u][0] = w.x;
         k[u][1] = w.y;
         k[u][DH / 32 - 2] = w.z;
         k[u][DH / 32 - 1] = w.w;
       } else {
-        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(c.codes[0] + r * (DH / 2)) + q);
+        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(src + u * 8 * (DH / 2)));
         k[u][0] = w.x;
         k[u][1] = w.y;
       }
-      km[u] = __ldcs(c.meta[0] + r * NB + (DH == 128 ? q >> 1 : 0));
+      km[u] = __ldcs(meta + u * 8 * (DH / 64));
     }
+  }
+  // rows 2 q4, + 1, + 8, + 9, this thread's eighth of the dims
+  __device__ __forceinline__ void load_v(int64_t row) {
+    const uint8_t *src = vc + row * (DH / 2);
+    const uint32_t *meta = vp + row * (DH / 64);
 #pragma unroll
     for (int u = 0; u < 4; u++) {
-      const int64_t r = row + 2 * q + (u & 1) + 8 * (u >> 1);
+      const int r = (u & 1) + 8 * (u >> 1);
       if (DH == 128) {
-        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(c.codes[1] + r * (DH / 2)) + n);
+        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(src + r * (DH / 2)));
         v[u][0] = w.x;
         v[u][DH / 64 - 1] = w.y;
       } else {
-        v[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(c.codes[1] + r * (DH / 2)) + n);
+        v[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(src + r * (DH / 2)));
       }
-      vm[u] = __ldcs(c.meta[1] + r * NB + (DH == 128 ? n >> 2 : 0));
+      vm[u] = __ldcs(meta + r * (DH / 64));
     }
   }
 };
@@ -217,12 +234,15 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(const AttendArgs a) {
     auto row_of = [&](int i, int pg) -> int64_t {
       return ((int64_t)pg * c.heads + kh) * c.page_size + (tiles.key0(i, 16) & (c.page_size - 1));
     };
-    TileRegs<DH> cur, next;
+    TileRegs<DH> cur(c, lane);
     int pg = page_of(t), pg_next = page_of(t + WARPS);
-    if (pg >= 0) cur.load(c, row_of(t, pg), lane);
+    if (pg >= 0) {
+      cur.load_k(row_of(t, pg));
+      cur.load_v(row_of(t, pg));
+    }
     for (; t < t1; t += WARPS) {
       const int pg_next2 = page_of(t + 2 * WARPS);
-      if (pg_next >= 0) next.load(c, row_of(t + WARPS, pg_next), lane);
+      const int64_t row_next = pg_next >= 0 ? row_of(t + WARPS, pg_next) : 0;
       if (pg >= 0) {
         const int key0 = tiles.key0(t, 16);
         // ---- scores: S^T (16 keys x 8 NT rows)
@@ -255,6 +275,7 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(const AttendArgs a) {
             for (int nt = 0; nt < NT; nt++) mma_bf16(sc[nt], fa, qf[nt][4 * w + 2 * h], qf[nt][4 * w + 2 * h + 1]);
           }
         }
+        if (pg_next >= 0) cur.load_k(row_next);   // K's registers are free again; V's after the second product
         // ---- mask; scores to log2 units.  sc[e]: key key0 + n8 + 8 (e >> 1), row 8 nt + 2 q4 + (e & 1)
         const bool all = key0 + 15 <= p_lo && (a.window == 0 || key0 > p_top - a.window || key0 + 15 < a.sinks);
         bool over = false;
@@ -332,7 +353,8 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(const AttendArgs a) {
           }
         }
       }
-      cur = next;
+      else if (pg_next >= 0) cur.load_k(row_next);
+      if (pg_next >= 0) cur.load_v(row_next);
       pg = pg_next;
       pg_next = pg_next2;
     }
@@ -856,46 +878,66 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
 
 }  // namespace tiles
 
-// The shares of a (row, query head), added in their order: a warp each.
+// The shares of a (row, query head), added in their order: a CTA each, four
+// warps with every fourth share and eight of them on their way at a time (the
+// chain of dependent loads is the time of this kernel), joined in shared
+// memory.
 template <int DH>
 __global__ void __launch_bounds__(128) attend_join_kernel(const AttendArgs a) {
+  constexpr int V = DH / 32;
+  __shared__ float so[4][DH];
+  __shared__ float2 sml[4];
   const CacheArgs &c = a.c;
-  const int heads = c.heads * a.group, lane = threadIdx.x & 31;
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5), all = c.rows * heads;
-  if (at >= all) return;
+  const int heads = c.heads * a.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t at = blockIdx.x, all = c.rows * heads;
   const int64_t token = at / heads;
   const int head = (int)(at - token * heads);
   if (token < c.cu_new[0] || token >= c.cu_new[c.B]) return;   // rows of no sequence stay as they are
-  constexpr int V = DH / 32;
-  float m = -INFINITY;
-  for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, a.part_ml[s * all + at].x);
+  // this warp's shares s = warp, warp + 4, ... (at most 16): lane k has the k-th one's reference and weight
+  const int mine = warp + 4 * lane;
+  const float2 ml = mine < a.splits ? a.part_ml[mine * all + at] : make_float2(-INFINITY, 0.0f);
+  float m = ml.x;
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-  float l = 0.0f, v[V];
+  const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m);   // nothing visible in a share: no part in the sum
+  float l = f * ml.y, v[V];
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
 #pragma unroll
   for (int k = 0; k < V; k++) v[k] = 0.0f;
-  for (int s = 0; s < a.splits; s++) {
-    const float2 ml = a.part_ml[s * all + at];
-    if (ml.x == -INFINITY) continue;   // nothing visible in this share
-    const float f = ex2(ml.x - m);
-    l += f * ml.y;
-    const float *src = a.part + (s * all + at) * DH + lane * V;
+#pragma unroll 8
+  for (int k = 0; k < (a.splits - warp + 3) / 4; k++) {
+    const float *src = a.part + ((warp + 4 * k) * all + at) * DH + lane * V;
+    const float w = __shfl_sync(0xffffffffu, f, k);
 #pragma unroll
-    for (int k = 0; k < V; k++) v[k] += f * src[k];
+    for (int e = 0; e < V; e++) v[e] += w == 0.0f ? 0.0f : w * src[e];
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint32_t *dst = reinterpret_cast<uint32_t *>(a.out + token * a.o_row + head * a.o_head + lane * V);
 #pragma unroll
-  for (int k = 0; k < V / 2; k++) dst[k] = pack_bf16(v[2 * k] * inv, v[2 * k + 1] * inv);
+  for (int e = 0; e < V; e++) so[warp][lane * V + e] = v[e];
+  if (lane == 0) sml[warp] = make_float2(m, l);
+  __syncthreads();
+  if (threadIdx.x >= DH / 2) return;
+  const int d = threadIdx.x * 2;
+  float top = -INFINITY, total = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; w++) top = fmaxf(top, sml[w].x);
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    const float g = sml[w].x == -INFINITY ? 0.0f : ex2(sml[w].x - top);
+    total += g * sml[w].y;
+    o0 += g * so[w][d];
+    o1 += g * so[w][d + 1];
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  *reinterpret_cast<uint32_t *>(a.out + token * a.o_row + head * a.o_head + d) = pack_bf16(o0 * inv, o1 * inv);
 }
 
-// Shares of the keys of one (sequence, key head): enough CTAs for four on
-// every SM, none with fewer than two tiles for each of its warps, and no more
+// Shares of the keys of one (sequence, key head): twelve CTAs for every SM, none with fewer than two tiles for each of its warps, and no more
 // than 2^26 partial sums (256 MB) in all.
 static int attend_splits(int sms, int64_t lanes, int64_t keys, int64_t outputs) {
-  const int64_t want = (4 * (int64_t)sms + lanes - 1) / lanes, most = std::max<int64_t>(1, keys / (16 * 4 * 2));
+  const int64_t want = (12 * (int64_t)sms + lanes - 1) / lanes, most = std::max<int64_t>(1, keys / (16 * 4 * 2));
   const int64_t room = (int64_t(1) << 26) / std::max<int64_t>(1, outputs);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, room, 256}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, room, MOST_SPLITS}));
 }
 
 // How a call is carried out: from its sizes alone.
@@ -937,7 +979,7 @@ static int attend_plan(const AttendSizes &z, AttendPlan *p) {
     // shares of the keys: as many as fill the SMs once, four steps or more to each
     const int64_t busy = std::max<int64_t>(1, z.rows * group / tiles::ROWS) * H;
     p->splits = (int)std::max<int64_t>(
-        1, std::min<int64_t>({sms / busy, keys / (4 * tiles::KEYS), (int64_t(1) << 26) / (z.rows * z.q_heads * z.head_dim), 64}));
+        1, std::min<int64_t>({sms / busy, keys / (4 * tiles::KEYS), (int64_t(1) << 26) / (z.rows * z.q_heads * z.head_dim), MOST_SPLITS}));
   } else {
     p->splits = attend_splits(sms, B * H, keys, z.rows * z.q_heads * z.head_dim);
   }
@@ -1043,7 +1085,7 @@ extern "C" int hif4x_paged_attention(const hif4x_kv_cache *kv, const hif4x_kv_ba
     HIF4X_CHECK_LAUNCH();
   }
   if (p.splits > 1) {
-    const unsigned blocks = (unsigned)((rows * q_heads + 3) / 4);
+    const unsigned blocks = (unsigned)(rows * q_heads);
     if (kv->head_dim == 128) attend_join_kernel<128><<<blocks, 128, 0, s>>>(a);
     else attend_join_kernel<64><<<blocks, 128, 0, s>>>(a);
     HIF4X_CHECK_LAUNCH();
