@@ -18,9 +18,17 @@
 
 namespace hif4x {
 
+// a b + c, kept a multiply-add: shifts and additions in its place would run on
+// the ALU pipe, which the masks fill
+__device__ __forceinline__ uint32_t mad32(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("mad.lo.u32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+
 // nibbles sign << 3 | m -> 8 + m or 8 - m (no carry leaves a nibble)
 __device__ __forceinline__ uint32_t hif4_offset(uint32_t w) {
-  const uint32_t neg7 = ((w >> 3) & 0x11111111u) * 7u;   // 7 in each negative nibble
+  const uint32_t neg7 = mad32((w >> 3) & 0x11111111u, 7u, 0u);   // 7 in each negative nibble
   return ((w & 0x77777777u) ^ neg7) + (0x88888888u - neg7);
 }
 
@@ -38,7 +46,7 @@ constexpr uint32_t kNeg136 = 0xc308c308u;   // bf16 pair -136
 
 // bf16 bits of sf/4 in both halves: the E6M2 byte (E + 48) << 2 | M is the
 // top of a bf16 significand, so its exponent is rebased by one addition
-__device__ __forceinline__ uint32_t hif4_sf2(uint32_t meta) { return (meta & 0xffu) * 0x00200020u + 0x26802680u; }
+__device__ __forceinline__ uint32_t hif4_sf2(uint32_t meta) { return mad32(meta & 0xffu, 0x00200020u, 0x26802680u); }
 
 // The lv bits of four sub-blocks i0 .. i0 + 3 of a group: bit j of l2, bits 2j
 // and 2j + 1 of l3.
@@ -52,9 +60,9 @@ struct Hif4Levels {
 template <int J>
 __device__ __forceinline__ void hif4_scales(const Hif4Levels &l, uint32_t sf2, uint32_t &s0, uint32_t &s1) {
   static_assert(J >= 0 && J < 4, "four sub-blocks");
-  const uint32_t b = (l.l2 & (1u << J)) * (0x00800080u >> J) + sf2;
-  s0 = (l.l3 & (1u << (2 * J))) * (0x00800080u >> (2 * J)) + b;
-  s1 = (l.l3 & (2u << (2 * J))) * (0x00800080u >> (2 * J + 1)) + b;
+  const uint32_t b = mad32(l.l2 & (1u << J), 0x00800080u >> J, sf2);
+  s0 = mad32(l.l3 & (1u << (2 * J)), 0x00800080u >> (2 * J), b);
+  s1 = mad32(l.l3 & (2u << (2 * J)), 0x00800080u >> (2 * J + 1), b);
 }
 
 // Word of sub-block i0 + J -> four bf16 pairs in element order (0,1) (2,3) (4,5) (6,7).

@@ -157,7 +157,7 @@ struct TileRegs {
 
 // DH: head dim; NT: query rows / 8 of a row tile.
 template <int DH, int NT>
-__global__ void __launch_bounds__(128) attend_rows_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) attend_rows_kernel(const AttendArgs a) {
   constexpr int WARPS = 4, KW = DH / 32, ROWS = 8 * NT;
   __shared__ float so[WARPS][ROWS][DH + 4];
   __shared__ float2 sml[WARPS][ROWS];
@@ -445,49 +445,70 @@ struct Cfg {
 // A warp's 16 keys of a K or V tile, packed in registers: lane -> (key of a
 // run of eight or sixteen, 16-byte chunk of 32 dims).
 template <int DH>
-struct Loader {
+struct Words {
   static constexpr int CPR = DH / 32;          // chunks per row
   static constexpr int KPI = 32 / CPR;         // keys per load
   static constexpr int N = 16 / KPI;           // loads
   uint4 w[N];
   uint32_t m[N];
-  bool have[N];
+};
 
-  static __device__ __forceinline__ int key(int lane) { return (lane & 7) + (CPR == 2 ? 8 * (lane >> 4) : 0); }
-  static __device__ __forceinline__ int chunk(int lane) { return CPR == 4 ? lane >> 3 : (lane >> 3) & 1; }
+template <int DH>
+struct Loader {
+  using W = Words<DH>;
+  int key, part;                  // key of a load, first sub-block of the lane's half group
+  uint32_t codes_at, meta_at;     // bytes from a 16-key block's first row
+  uint32_t page_codes, page_meta; // bytes of a page (all heads)
+  uint32_t head_codes, head_meta; // bytes to this head's rows in it
+  int slots;                      // page_size - 1
+  uint32_t to;                    // byte of the lane's first row in a tile
 
-  // keys first .. first + 15, all of page `page` (negative: none); behind `last` there are none
-  __device__ __forceinline__ void load(const CacheArgs &c, int which, int kh, int first, int page, int last, int lane) {
-    const int64_t row = ((int64_t)max(page, 0) * c.heads + kh) * c.page_size + (first & (c.page_size - 1)) + key(lane);
-    const uint4 *src = reinterpret_cast<const uint4 *>(c.codes[which] + row * (DH / 2)) + chunk(lane);
-    const uint32_t *meta = c.meta[which] + row * (DH / 64) + (CPR == 4 ? chunk(lane) >> 1 : 0);
+  __device__ __forceinline__ Loader(const CacheArgs &c, int kh, int warp, int lane) {
+    const int chunk = W::CPR == 4 ? lane >> 3 : (lane >> 3) & 1;
+    key = (lane & 7) + (W::CPR == 2 ? 8 * (lane >> 4) : 0);
+    part = (chunk & 1) * 4;
+    codes_at = key * (DH / 2) + chunk * 16;
+    meta_at = (key * (DH / 64) + (W::CPR == 4 ? chunk >> 1 : 0)) * 4;
+    page_codes = (uint32_t)c.heads * c.page_size * (DH / 2);
+    page_meta = (uint32_t)c.heads * c.page_size * (DH / 64) * 4;
+    head_codes = (uint32_t)kh * c.page_size * (DH / 2);
+    head_meta = (uint32_t)kh * c.page_size * (DH / 64) * 4;
+    slots = c.page_size - 1;
+    to = (W::CPR == 4 ? (chunk >> 1) * Cfg<DH>::PANEL : 0) + (warp * 16 + key) * 128;
+  }
+  // keys first .. first + 15, all of page `page`.  Where there is none (negative) page 0's are taken, and keys
+  // behind the last come as they lie there: every bit pattern decodes to a finite value, and their scores are
+  // masked, so nothing of them reaches a result.
+  __device__ __forceinline__ void load(W &x, const uint8_t *codes, const uint32_t *meta, int first, int page) const {
+    const uint32_t p = (uint32_t)max(page, 0), slot = (uint32_t)(first & slots);
+    const uint8_t *src = codes + (uint64_t)p * page_codes + (head_codes + slot * (DH / 2) + codes_at);
+    const uint8_t *msrc = reinterpret_cast<const uint8_t *>(meta) + (uint64_t)p * page_meta + (head_meta + slot * (DH / 16) + meta_at);
 #pragma unroll
-    for (int it = 0; it < N; it++) {
-      w[it] = __ldg(src + it * KPI * (DH / 32));
-      m[it] = __ldg(meta + it * KPI * (DH / 64));
-      have[it] = page >= 0 && first + it * KPI + key(lane) <= last;
+    for (int it = 0; it < W::N; it++) {
+      x.w[it] = __ldg(reinterpret_cast<const uint4 *>(src + it * W::KPI * (DH / 2)));
+      x.m[it] = __ldg(reinterpret_cast<const uint32_t *>(msrc + it * W::KPI * (DH / 16)));
     }
   }
   // decoded into a tile: panel of 64 dims, key rows of 128 bytes, 16-byte chunk q at q ^ (key & 7); inside a
   // chunk the dims stand as (0 2 4 6 1 3 5 7), as Q's do
-  __device__ __forceinline__ void store(uint8_t *tile, int warp, int lane) const {
-    const int ch = chunk(lane), q0 = (ch & 1) * 4;   // first sub-block of the group = 16-byte chunk of the panel row
+  __device__ __forceinline__ void store(const W &x, uint8_t *tile) const {
+    uint8_t *row = tile + to;
+    const int swz = key & 7;
 #pragma unroll
-    for (int it = 0; it < N; it++) {
-      const int k = warp * 16 + it * KPI + key(lane);
-      uint8_t *row = tile + (CPR == 4 ? (ch >> 1) * Cfg<DH>::PANEL : 0) + k * 128;
-      const uint32_t mm = have[it] ? m[it] : 0u, sf2 = hif4_sf2(mm);
-      const Hif4Levels l(mm, q0);
-      const uint4 c = have[it] ? w[it] : make_uint4(0, 0, 0, 0);   // code 0 decodes to 0
+    for (int it = 0; it < W::N; it++) {
+      const uint32_t sf2 = hif4_sf2(x.m[it]);
+      const Hif4Levels l(x.m[it], part);
+      const uint4 c = x.w[it];
+      uint8_t *at = row + it * W::KPI * 128;
       uint32_t o[4];
       hif4_decode8_even_odd<0>(c.x, l, sf2, o);
-      *reinterpret_cast<uint4 *>(row + ((q0 ^ (k & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4 *>(at + ((part ^ swz) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
       hif4_decode8_even_odd<1>(c.y, l, sf2, o);
-      *reinterpret_cast<uint4 *>(row + (((q0 + 1) ^ (k & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4 *>(at + (((part + 1) ^ swz) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
       hif4_decode8_even_odd<2>(c.z, l, sf2, o);
-      *reinterpret_cast<uint4 *>(row + (((q0 + 2) ^ (k & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4 *>(at + (((part + 2) ^ swz) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
       hif4_decode8_even_odd<3>(c.w, l, sf2, o);
-      *reinterpret_cast<uint4 *>(row + (((q0 + 3) ^ (k & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4 *>(at + (((part + 3) ^ swz) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   }
 };
@@ -643,7 +664,8 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
     const int last = p_hi;
     // item u: K (even) or V (odd) of step u / 2; the next one's words are on their way meanwhile, and so is what
     // the page table says of the step after
-    Loader<DH> cur, next;
+    const Loader<DH> ld(c, kh, w, lane);
+    Words<DH> cur, next;
     auto key_of = [&](int i) { return kt.key0(first + i, KEYS) + w * 16; };
     auto look = [&](int i) { return i < n && key_of(i) <= last ? __ldg(pages + (key_of(i) >> c.page_shift)) : -1; };
     auto check = [&](int i, int page) {   // an id of no page: -1, and reported where the keys exist
@@ -653,22 +675,22 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
     };
     int now = look(0), nxt = look(1);   // of the step being decoded, of the one after it
     now = check(0, now);
-    if (n > 0) cur.load(c, 0, kh, key_of(0), now, last, lane);
+    if (n > 0) ld.load(cur, c.codes[0], c.meta[0], key_of(0), now);
 #pragma unroll 1
     for (int u = 0; u < 2 * n; u++) {
       const int i = u >> 1, v = u & 1, s = i & 1;
       if (v == 0) {
-        next.load(c, 1, kh, key_of(i), now, last, lane);
+        ld.load(next, c.codes[1], c.meta[1], key_of(i), now);
         if (lane == 0) hidden[(i & 3) * 8 + w] = now < 0 ? 1 : 0;
       } else if (i + 1 < n) {
         now = check(i + 1, nxt);
-        next.load(c, 0, kh, key_of(i + 1), now, last, lane);
+        ld.load(next, c.codes[0], c.meta[0], key_of(i + 1), now);
         nxt = look(i + 2);
       }
       if (i >= 2) ok = mbar_wait_sleep((v ? vempty : kempty) + s, ((i >> 1) - 1) & 1, c.status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      cur.store(smem + (v ? C::V : C::K) + s * C::TILE, w, lane);
+      ld.store(cur, smem + (v ? C::V : C::K) + s * C::TILE);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive((v ? vfull : kfull) + s);
@@ -932,10 +954,17 @@ __global__ void __launch_bounds__(128) attend_join_kernel(const AttendArgs a) {
   *reinterpret_cast<uint32_t *>(a.out + token * a.o_row + head * a.o_head + d) = pack_bf16(o0 * inv, o1 * inv);
 }
 
-// Shares of the keys of one (sequence, key head): twelve CTAs for every SM, none with fewer than two tiles for each of its warps, and no more
-// than 2^26 partial sums (256 MB) in all.
-static int attend_splits(int sms, int64_t lanes, int64_t keys, int64_t outputs) {
-  const int64_t want = (12 * (int64_t)sms + lanes - 1) / lanes, most = std::max<int64_t>(1, keys / (16 * 4 * 2));
+// Shares of the keys of one (sequence, key head) in attend_rows_kernel.  Few
+// lanes (sequence, key head): as many shares as the SMs hold CTAs at once (a
+// second wave would leave most of them idle; 65536 keys of one sequence: 50
+// us, 91 with three waves).  Many: twelve CTAs for every SM, so that sequences
+// of several lengths even out (64 sequences of up to 8192 keys: 180 us, 289
+// unshared).  No share under two tiles for each warp, and no more than 2^26
+// partial sums (256 MB) in all.
+static int attend_splits(int sms, int64_t lanes, int64_t keys, int64_t outputs, bool two) {
+  const int64_t at_once = (two ? 2 : 3) * (int64_t)sms;
+  const int64_t want = lanes * 4 <= at_once * 3 ? at_once / lanes : (12 * (int64_t)sms + lanes - 1) / lanes;
+  const int64_t most = std::max<int64_t>(1, keys / (16 * 4 * 2));
   const int64_t room = (int64_t(1) << 26) / std::max<int64_t>(1, outputs);
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, room, MOST_SPLITS}));
 }
@@ -981,7 +1010,7 @@ static int attend_plan(const AttendSizes &z, AttendPlan *p) {
     p->splits = (int)std::max<int64_t>(
         1, std::min<int64_t>({sms / busy, keys / (4 * tiles::KEYS), (int64_t(1) << 26) / (z.rows * z.q_heads * z.head_dim), MOST_SPLITS}));
   } else {
-    p->splits = attend_splits(sms, B * H, keys, z.rows * z.q_heads * z.head_dim);
+    p->splits = attend_splits(sms, B * H, keys, z.rows * z.q_heads * z.head_dim, (int64_t)z.max_new * group > 8);
   }
   p->part_floats = p->splits > 1 ? (int64_t)p->splits * z.rows * z.q_heads * z.head_dim : 0;
   p->work_bytes = p->splits > 1 ? p->part_floats * 4 + (int64_t)p->splits * z.rows * z.q_heads * 8 : 0;
