@@ -12,13 +12,15 @@
 //   warp 0   one lane brings x tiles (NT x 64) by TMA, 128-byte swizzle
 //   warp 1   one lane issues tcgen05.mma kind::f16 (M 128, N NT, K 16)
 //   warp 2   one lane brings W's codes by TMA, 128 rows x 256 elements (16 KB)
-//   warps 4-11  two warpgroups decode the 64-element steps in turn: a thread
+//   warps 4-19  four warpgroups decode the 64-element steps in turn: a thread
 //            is one row of W, reads its 32 bytes and one meta word, and writes
 //            32 columns of bf16 pairs to tensor memory, where the MMA reads A
-//            from.  W's tile never passes shared memory as bf16: that leaves
+//            from.  (A decoding warp alone issues an instruction in 5 to 6
+//            cycles: with two warps a scheduler a step took 830 cycles, with
+//            four XXXX; the ALU pipe's floor is 270.)  W's tile never passes shared memory as bf16: that leaves
 //            shared memory's bandwidth to x alone (a 128 x 256 x 64 step would
 //            otherwise write and read 96 KB there, more than its MMA time).
-// C is shared out over a cluster of up to 8 CTAs where the tiles alone do not
+// C is shared out over a cluster of up to 4 CTAs where the tiles alone do not
 // fill the GPU; the partial sums meet through distributed shared memory and
 // are added in rank order, so results do not depend on timing.
 // Every wait is bounded (sm100.cuh); on expiry the kernel records
@@ -37,8 +39,9 @@ using namespace tc;
 constexpr int STAGES = 4;        // 64-element steps of x and of decoded W in flight
 constexpr int CODE_STAGES = 3;   // 256-element boxes of packed W in flight
 constexpr int CODE_BYTES = 128 * 128;
-constexpr int THREADS = 384;
+constexpr int THREADS = 640;
 constexpr int BM = 128;
+constexpr int MOST_RANKS = 4;    // CTAs of a cluster that share a tile's C (clusters of 8 do not fit every GPC twice)
 
 struct Args {
   int64_t T, N;
@@ -110,7 +113,7 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
     }
     for (int s = 0; s < CODE_STAGES; s++) {
       mbar_init(&full_w[s], 1);
-      mbar_init(&empty_w[s], 8);
+      mbar_init(&empty_w[s], 16);
     }
     mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -174,55 +177,53 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
         if (i > s) mbar_wait_limit(&full_w[s], ((i - 1 - s) / CODE_STAGES) & 1, SPIN_LIMIT, a.status);
     }
   } else if (warp >= 4) {
-    // ---- decode: thread = row of W (tensor memory lane), steps of this warpgroup's parity
-    const int wg = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
+    // ---- decode: thread = row of W (tensor memory lane); warpgroup g has group g of every box, stage g
+    const int g = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
     const int64_t row = row0 + r;
-    const uint32_t *meta = a.meta + (row < a.N ? row : 0) * a.nb + k0;
+    const uint32_t *meta = a.meta + (row < a.N ? row : 0) * a.nb + k0 + g;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const int boxes = (steps + 3) / 4;
-    uint32_t m0 = wg < steps ? __ldg(meta + wg) : 0u, m1 = 2 + wg < steps ? __ldg(meta + 2 + wg) : 0u;
+    // 16-byte chunk c of row r lies at chunk c ^ (r & 7)
+    const uint8_t *src0 = sw + r * 128 + (((2 * g) ^ (r & 7)) << 4), *src1 = sw + r * 128 + (((2 * g + 1) ^ (r & 7)) << 4);
+    const int boxes = (steps + 3) / 4, mine = (steps - g + 3) / 4;   // this warpgroup's steps: the first boxes
+    uint32_t m = mine > 0 ? __ldg(meta) : 0u;
+    int cs = 0, cp = 0;   // code stage and its phase
     for (int b = 0; b < boxes && ok; b++) {
-      const int cs = b % CODE_STAGES, nx = 4 * (b + 1) + wg;
-      const uint32_t n0 = nx < steps ? __ldg(meta + nx) : 0u, n1 = nx + 2 < steps ? __ldg(meta + nx + 2) : 0u;
-      ok = mbar_wait_limit(&full_w[cs], (b / CODE_STAGES) & 1, SPIN_LIMIT, a.status);
+      const uint32_t next = b + 1 < mine ? __ldg(meta + 4 * (b + 1)) : 0u;
+      ok = mbar_wait_limit(&full_w[cs], cp, SPIN_LIMIT, a.status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      const uint8_t *src = sw + cs * CODE_BYTES + r * 128;
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int g = 2 * h + wg, i = 4 * b + g;   // group of the box, step
-        if (i >= steps) break;
-        const uint32_t m = h ? m1 : m0;
-        // 16-byte chunk c of row r lies at chunk c ^ (r & 7)
-        const uint4 c0 = *reinterpret_cast<const uint4 *>(src + (((2 * g) ^ (r & 7)) << 4));
-        const uint4 c1 = *reinterpret_cast<const uint4 *>(src + (((2 * g + 1) ^ (r & 7)) << 4));
+      const uint4 c0 = *reinterpret_cast<const uint4 *>(src0 + cs * CODE_BYTES);
+      const uint4 c1 = *reinterpret_cast<const uint4 *>(src1 + cs * CODE_BYTES);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty_w[cs]);
+      if (++cs == CODE_STAGES) {
+        cs = 0;
+        cp ^= 1;
+      }
+      if (b < mine) {
         const uint32_t w[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
         uint32_t v[32];
         hif4_decode64(w, m, v);
-        const int s = i % STAGES;
-        if (i >= STAGES) {
-          ok = mbar_wait_limit(&empty[s], ((i / STAGES) - 1) & 1, SPIN_LIMIT, a.status);
+        if (b > 0) {
+          ok = mbar_wait_limit(&empty[g], (b - 1) & 1, SPIN_LIMIT, a.status);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
         }
-        tmem_st32(tmem_a + lanes + s * 32, v);
+        tmem_st32(tmem_a + lanes + g * 32, v);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full_a[s]);
+        if (lane == 0) mbar_arrive(&full_a[g]);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty_w[cs]);
-      m0 = n0;
-      m1 = n1;
+      m = next;
     }
     // ---- the accumulator to shared memory, [x row][row of W], over the x stages
     ok = mbar_wait_limit(done, 0, SPIN_LIMIT, a.status);
     __syncwarp();
     tc_fence_after();
     float *part = reinterpret_cast<float *>(sx);
-    for (int n = wg * 16; n < a.nt; n += 32) {
+    for (int n = g * 16; n < a.nt; n += 64) {
       uint32_t d[16];
       if (steps > 0) {
         tmem_ld16(tmem_d + lanes + n, d);
@@ -252,14 +253,25 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
     if (n >= a.N) continue;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     const uint32_t at = base + (uint32_t)(t * BM + c) * 4u;
-    for (int z = 0; z < ranks; z++) {
-      const uint32_t from = ranks > 1 ? mapa(at, z) : at;
-      const float4 p = ld_cluster4(from), q = ld_cluster4(from + 16);
-      v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
-      v[4] += q.x; v[5] += q.y; v[6] += q.z; v[7] += q.w;
-    }
     const int64_t tok = tok0 + t;
     const int m = (int)min((int64_t)8, a.N - n);
+    const bool wide = a.vec && m == 8;
+    uint4 res = make_uint4(0, 0, 0, 0);   // on its way while the sums are read
+    if (wide && a.res != nullptr) res = *reinterpret_cast<const uint4 *>(a.res + tok * a.ldr + n);
+    float4 p[MOST_RANKS], q[MOST_RANKS];
+#pragma unroll
+    for (int z = 0; z < MOST_RANKS; z++)
+      if (z < ranks) {
+        const uint32_t from = ranks > 1 ? mapa(at, z) : at;
+        p[z] = ld_cluster4(from);
+        q[z] = ld_cluster4(from + 16);
+      }
+#pragma unroll
+    for (int z = 0; z < MOST_RANKS; z++)
+      if (z < ranks) {
+        v[0] += p[z].x; v[1] += p[z].y; v[2] += p[z].z; v[3] += p[z].w;
+        v[4] += q[z].x; v[5] += q[z].y; v[6] += q[z].z; v[7] += q[z].w;
+      }
     if (a.bias != nullptr) {
 #pragma unroll
       for (int k = 0; k < 8; k++)
@@ -272,10 +284,9 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
       for (int k = 0; k < 8; k++) v[k] = activate(v[k], a.act);
     }
     uint16_t *dst = a.y + tok * a.ldy + n;
-    if (a.vec && m == 8) {
+    if (wide) {
       if (a.res != nullptr) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(a.res + tok * a.ldr + n);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        const uint32_t w[4] = {res.x, res.y, res.z, res.w};
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           v[2 * k] += __uint_as_float(w[k] << 16);
@@ -354,9 +365,9 @@ extern "C" int hif4x_linear_packed(const void *x, int64_t ldx, const uint32_t *m
   const int64_t tiles_n = (N + BM - 1) / BM;
   if (tiles_t > 65535) return HIF4X_ERR_UNSUPPORTED;
   a.nb = (int)(C / 64);
-  // share C out until there is a CTA for every SM, 4 steps or more to each
+  // share C out while that gives more SMs a CTA, 4 steps or more to each
   int ranks = 1;
-  while (ranks < 8 && tiles_n * tiles_t * ranks * 2 <= sms + sms / 4 && a.nb >= 8 * ranks) ranks *= 2;
+  while (ranks < MOST_RANKS && tiles_n * tiles_t * ranks * 2 <= sms && a.nb >= 8 * ranks) ranks *= 2;
   a.per = (int)(((a.nb + ranks - 1) / ranks + 3) / 4 * 4);
   a.T = T;
   a.N = N;
