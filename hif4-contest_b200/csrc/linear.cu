@@ -17,7 +17,7 @@
 //            32 columns of bf16 pairs to tensor memory, where the MMA reads A
 //            from.  (A decoding warp alone issues an instruction in 5 to 6
 //            cycles: with two warps a scheduler a step took 830 cycles, with
-//            four XXXX; the ALU pipe's floor is 270.)  W's tile never passes shared memory as bf16: that leaves
+//            four 600, of which the ALU pipe is busy for 330.)  W's tile never passes shared memory as bf16: that leaves
 //            shared memory's bandwidth to x alone (a 128 x 256 x 64 step would
 //            otherwise write and read 96 KB there, more than its MMA time).
 // C is shared out over a cluster of up to 4 CTAs where the tiles alone do not
@@ -36,8 +36,10 @@ namespace lin {
 
 using namespace tc;
 
-constexpr int STAGES = 4;        // 64-element steps of x and of decoded W in flight
+constexpr int MOST_X = 8;        // 64-element steps of x in flight, as shared memory allows (5 at least)
 constexpr int CODE_STAGES = 3;   // 256-element boxes of packed W in flight
+constexpr int PAIRS = 4;         // pairs of steps of decoded W in tensor memory, one for each warpgroup
+constexpr int SMEM = 231424;     // of a CTA, with barriers and alignment
 constexpr int CODE_BYTES = 128 * 128;
 constexpr int THREADS = 640;
 constexpr int BM = 128;
@@ -54,7 +56,7 @@ struct Args {
   uint16_t *y;
   int64_t ldy;
   int vec;                  // rows of y and residual take 16-byte accesses
-  uint32_t tmem_cols;
+  int xs;                   // stages of x
   int *status;
 };
 
@@ -94,10 +96,10 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int x_bytes = a.nt * 128;
-  uint8_t *sx = smem, *sw = smem + STAGES * x_bytes;
-  uint64_t *full_x = reinterpret_cast<uint64_t *>(sw + CODE_STAGES * CODE_BYTES);
-  uint64_t *full_a = full_x + STAGES, *empty = full_a + STAGES, *full_w = empty + STAGES;
-  uint64_t *empty_w = full_w + CODE_STAGES, *done = empty_w + CODE_STAGES;
+  uint8_t *sx = smem, *sw = smem + a.xs * x_bytes;
+  uint64_t *full_x = reinterpret_cast<uint64_t *>(sw + CODE_STAGES * CODE_BYTES), *empty_x = full_x + MOST_X;
+  uint64_t *full_a = empty_x + MOST_X, *empty_a = full_a + PAIRS;
+  uint64_t *full_w = empty_a + PAIRS, *empty_w = full_w + CODE_STAGES, *done = empty_w + CODE_STAGES;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -106,14 +108,17 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
   const int k0 = min(a.nb, rank * a.per), steps = min(a.nb, k0 + a.per) - k0;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; s++) {
+    for (int s = 0; s < a.xs; s++) {
       mbar_init(&full_x[s], 1);
+      mbar_init(&empty_x[s], 1);
+    }
+    for (int s = 0; s < PAIRS; s++) {
       mbar_init(&full_a[s], 4);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty_a[s], 1);
     }
     for (int s = 0; s < CODE_STAGES; s++) {
       mbar_init(&full_w[s], 1);
-      mbar_init(&empty_w[s], 16);
+      mbar_init(&empty_w[s], 8);
     }
     mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -121,44 +126,54 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
   if (warp == 1) {
     __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(a.tmem_cols));
+                 "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_a = *tmem_slot, tmem_d = tmem_a + STAGES * 32;   // A stages, then the accumulator
+  const uint32_t tmem_a = *tmem_slot, tmem_d = tmem_a + PAIRS * 64;   // decoded W, then the accumulator (256 columns)
   bool ok = true;
 
   if (warp == 0) {
     if (elect_one()) {
-      int i = 0;
+      int i = 0, s = 0, ph = 1;
       for (; i < steps; i++) {
-        const int s = i % STAGES;
-        if (i >= STAGES) ok = mbar_wait_limit(&empty[s], ((i / STAGES) - 1) & 1, SPIN_LIMIT, a.status);
+        if (i >= a.xs) ok = mbar_wait_sleep(&empty_x[s], ph, a.status);
         if (!ok) break;
         mbar_expect_tx(&full_x[s], x_bytes);
         tma_load_2d(&map_x, sx + s * x_bytes, &full_x[s], (k0 + i) * 64, (int)tok0);
+        if (++s == a.xs) {
+          s = 0;
+          ph ^= 1;
+        }
       }
       // no copy may be in flight when the CTA ends
-      for (int s = 0; s < STAGES; s++)
-        if (i > s) mbar_wait_limit(&full_x[s], ((i - 1 - s) / STAGES) & 1, SPIN_LIMIT, a.status);
+      for (int k = max(0, i - a.xs); k < i; k++) mbar_wait_sleep(&full_x[k % a.xs], (k / a.xs) & 1, a.status);
     }
   } else if (warp == 1) {
     if (elect_one()) {
       const uint32_t idesc = idesc_bf16((uint32_t)a.nt, 0);
       const uint64_t dx = smem_desc(smem_u32(sx), 16u, 1024u, 2u);   // + 2 for 32 bytes further
-      for (int i = 0; i < steps; i++) {
-        const int s = i % STAGES, ph = (i / STAGES) & 1;
-        ok = mbar_wait_limit(&full_x[s], ph, SPIN_LIMIT, a.status) &&
-             mbar_wait_limit(&full_a[s], ph, SPIN_LIMIT, a.status);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t x = dx + (uint32_t)(s * x_bytes >> 4);
+      int s = 0, ph = 0;
+      for (int i = 0; i < steps && ok; i += 2) {   // a warpgroup's pair of steps
+        const int g = (i >> 1) & 3;
+        ok = mbar_wait_sleep(&full_a[g], (i >> 3) & 1, a.status);
+        for (int u = i; u < min(i + 2, steps) && ok; u++) {
+          ok = mbar_wait_sleep(&full_x[s], ph, a.status);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t x = dx + (uint32_t)(s * x_bytes >> 4);
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          mma_f16_ts(tmem_d, tmem_a + s * 32 + j * 8, x + 2 * j, idesc, (i > 0 || j > 0) ? 1u : 0u);
-        mma_commit(&empty[s]);
+          for (int j = 0; j < 4; j++)
+            mma_f16_ts(tmem_d, tmem_a + g * 64 + (u & 1) * 32 + j * 8, x + 2 * j, idesc, (u > 0 || j > 0) ? 1u : 0u);
+          mma_commit(&empty_x[s]);
+          if (++s == a.xs) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        mma_commit(&empty_a[g]);
       }
       mma_commit(done);
     }
@@ -168,58 +183,64 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
       int i = 0;
       for (; i < boxes; i++) {
         const int s = i % CODE_STAGES;
-        if (i >= CODE_STAGES) ok = mbar_wait_limit(&empty_w[s], ((i / CODE_STAGES) - 1) & 1, SPIN_LIMIT, a.status);
+        if (i >= CODE_STAGES) ok = mbar_wait_sleep(&empty_w[s], ((i / CODE_STAGES) - 1) & 1, a.status);
         if (!ok) break;
         mbar_expect_tx(&full_w[s], CODE_BYTES);
         tma_load_2d(&map_w, sw + s * CODE_BYTES, &full_w[s], (k0 + 4 * i) * 32, (int)row0);
       }
       for (int s = 0; s < CODE_STAGES; s++)
-        if (i > s) mbar_wait_limit(&full_w[s], ((i - 1 - s) / CODE_STAGES) & 1, SPIN_LIMIT, a.status);
+        if (i > s) mbar_wait_sleep(&full_w[s], ((i - 1 - s) / CODE_STAGES) & 1, a.status);
     }
   } else if (warp >= 4) {
-    // ---- decode: thread = row of W (tensor memory lane); warpgroup g has group g of every box, stage g
+    // ---- decode: thread = row of W (tensor memory lane); of every eight steps warpgroup g has 2 g and 2 g + 1,
+    // the half g & 1 of every other box
     const int g = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
     const int64_t row = row0 + r;
-    const uint32_t *meta = a.meta + (row < a.N ? row : 0) * a.nb + k0 + g;
+    const uint32_t *meta = a.meta + (row < a.N ? row : 0) * a.nb + k0 + 2 * g;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    // 16-byte chunk c of row r lies at chunk c ^ (r & 7)
-    const uint8_t *src0 = sw + r * 128 + (((2 * g) ^ (r & 7)) << 4), *src1 = sw + r * 128 + (((2 * g + 1) ^ (r & 7)) << 4);
-    const int boxes = (steps + 3) / 4, mine = (steps - g + 3) / 4;   // this warpgroup's steps: the first boxes
-    uint32_t m = mine > 0 ? __ldg(meta) : 0u;
-    int cs = 0, cp = 0;   // code stage and its phase
-    for (int b = 0; b < boxes && ok; b++) {
-      const uint32_t next = b + 1 < mine ? __ldg(meta + 4 * (b + 1)) : 0u;
-      ok = mbar_wait_limit(&full_w[cs], cp, SPIN_LIMIT, a.status);
+    const int boxes = (steps + 3) / 4;
+    auto meta_of = [&](int t, int u) { return 8 * t + 2 * g + u < steps ? __ldg(meta + 8 * t + u) : 0u; };
+    uint32_t m0 = meta_of(0, 0), m1 = meta_of(0, 1), n0 = meta_of(1, 0), n1 = meta_of(1, 1);
+    for (int t = 0, b = g >> 1; b < boxes; t++, b += 2) {
+      const uint32_t o0 = meta_of(t + 2, 0), o1 = meta_of(t + 2, 1);
+      const int cs = b % CODE_STAGES;
+      ok = mbar_wait_sleep(&full_w[cs], (b / CODE_STAGES) & 1, a.status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      const uint4 c0 = *reinterpret_cast<const uint4 *>(src0 + cs * CODE_BYTES);
-      const uint4 c1 = *reinterpret_cast<const uint4 *>(src1 + cs * CODE_BYTES);
+      // 16-byte chunk c of row r lies at chunk c ^ (r & 7)
+      const uint8_t *src = sw + cs * CODE_BYTES + r * 128;
+      uint4 c[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) c[k] = *reinterpret_cast<const uint4 *>(src + (((4 * (g & 1) + k) ^ (r & 7)) << 4));
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty_w[cs]);
-      if (++cs == CODE_STAGES) {
-        cs = 0;
-        cp ^= 1;
-      }
-      if (b < mine) {
-        const uint32_t w[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+      if (8 * t + 2 * g >= steps) break;   // behind the last step
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const uint32_t w[8] = {c[2 * u].x,     c[2 * u].y,     c[2 * u].z,     c[2 * u].w,
+                               c[2 * u + 1].x, c[2 * u + 1].y, c[2 * u + 1].z, c[2 * u + 1].w};
         uint32_t v[32];
-        hif4_decode64(w, m, v);
-        if (b > 0) {
-          ok = mbar_wait_limit(&empty[g], (b - 1) & 1, SPIN_LIMIT, a.status);
+        hif4_decode64(w, u ? m1 : m0, v);
+        if (u == 0 && t > 0) {
+          ok = mbar_wait_sleep(&empty_a[g], (t - 1) & 1, a.status);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
         }
-        tmem_st32(tmem_a + lanes + g * 32, v);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full_a[g]);
+        tmem_st32(tmem_a + lanes + g * 64 + u * 32, v);
       }
-      m = next;
+      if (!ok) break;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full_a[g]);
+      m0 = n0;
+      m1 = n1;
+      n0 = o0;
+      n1 = o1;
     }
     // ---- the accumulator to shared memory, [x row][row of W], over the x stages
-    ok = mbar_wait_limit(done, 0, SPIN_LIMIT, a.status);
+    ok = mbar_wait_sleep(done, 0, a.status);
     __syncwarp();
     tc_fence_after();
     float *part = reinterpret_cast<float *>(sx);
@@ -241,7 +262,7 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_a), "r"(a.tmem_cols));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_a), "r"(512));
   }
   if (ranks > 1) cluster_sync();
   // ---- the ranks' sums, bias, activation, residual: 8 outputs of one x row a thread
@@ -326,10 +347,6 @@ static bool map_rows(CUtensorMap *map, CUtensorMapDataType type, const void *bas
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-static int smem_bytes(int nt) {
-  return STAGES * nt * 128 + CODE_STAGES * CODE_BYTES + (3 * STAGES + 2 * CODE_STAGES + 1) * 8 + 16 + 1024;
-}
-
 }  // namespace lin
 }  // namespace hif4x
 
@@ -352,17 +369,30 @@ extern "C" int hif4x_linear_packed(const void *x, int64_t ldx, const uint32_t *m
   static std::once_flag once[kMaxDevices];
   static bool attr_ok[kMaxDevices];
   std::call_once(once[dev], [dev] {
-    attr_ok[dev] = cudaFuncSetAttribute(linear_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(256)) ==
+    attr_ok[dev] = cudaFuncSetAttribute(linear_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) ==
                    cudaSuccess;
   });
   Args a{};
   a.status = status_word(dev);
   if (!attr_ok[dev] || !a.status) return HIF4X_ERR_LAUNCH;
 
-  // x rows of a tile: as few tiles as possible, alike
-  const int64_t tiles_t = (T + 255) / 256;
-  a.nt = (int)(((T + tiles_t - 1) / tiles_t + 15) / 16 * 16);
   const int64_t tiles_n = (N + BM - 1) / BM;
+  // x rows of a tile, all tiles alike: of the tilings from the fewest tiles on, the one whose waves of CTAs take
+  // least, a step taking 2.25 cycles a row (shared memory: x in and out) and never under 600 (decoding).
+  // 4096 x 4096 rows: 18 tiles of 240, four waves, instead of 16 of 256, four waves too
+  const int64_t fewest = (T + 255) / 256;
+  int64_t tiles_t = fewest, least = INT64_MAX;
+  for (int64_t n = fewest; n <= fewest + fewest / 4; n++) {
+    const int64_t nt = ((T + n - 1) / n + 15) / 16 * 16;
+    const int64_t cost = ((tiles_n * n + sms - 1) / sms) * std::max<int64_t>(600 * 4, 9 * nt);
+    if (cost < least) {
+      least = cost;
+      tiles_t = n;
+    }
+    if (n - fewest >= 64) break;
+  }
+  a.nt = (int)(((T + tiles_t - 1) / tiles_t + 15) / 16 * 16);
+  tiles_t = (T + a.nt - 1) / a.nt;
   if (tiles_t > 65535) return HIF4X_ERR_UNSUPPORTED;
   a.nb = (int)(C / 64);
   // share C out while that gives more SMs a CTA, 4 steps or more to each
@@ -381,7 +411,7 @@ extern "C" int hif4x_linear_packed(const void *x, int64_t ldx, const uint32_t *m
   a.ldy = ldy;
   a.vec = (reinterpret_cast<uintptr_t>(y) & 15u) == 0 && ldy % 8 == 0 &&
           (!residual || ((reinterpret_cast<uintptr_t>(residual) & 15u) == 0 && ldr % 8 == 0));
-  a.tmem_cols = a.nt <= 128 ? 256u : 512u;
+  a.xs = std::min(MOST_X, (SMEM - 1024 - 512 - CODE_STAGES * CODE_BYTES) / (a.nt * 128));
   CUtensorMap mx, mw;
   if (!map_rows(&mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, C, T, ldx * 2, 64, a.nt) ||
       !map_rows(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, C / 2, N, C / 2, 128, BM))
@@ -389,7 +419,7 @@ extern "C" int hif4x_linear_packed(const void *x, int64_t ldx, const uint32_t *m
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)tiles_n, (unsigned)tiles_t, (unsigned)ranks);
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem_bytes(a.nt);
+  cfg.dynamicSmemBytes = a.xs * a.nt * 128 + CODE_STAGES * CODE_BYTES + 512 + 1024;
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;

@@ -55,7 +55,7 @@ __device__ __forceinline__ bool mbar_wait_limit(uint64_t *bar, uint32_t parity, 
 // The same with a hint that the thread may sleep up to a microsecond a poll:
 // warps of other roles on the scheduler then lose fewer issue slots to polling.
 __device__ __forceinline__ bool mbar_wait_sleep(uint64_t *bar, uint32_t parity, int *status) {
-  for (long long i = 0; i < SPIN_LIMIT; i++) {
+  for (int i = 0; i < (int)SPIN_LIMIT; i++) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
