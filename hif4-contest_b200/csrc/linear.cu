@@ -37,7 +37,8 @@ namespace lin {
 using namespace tc;
 
 constexpr int MOST_X = 8;        // 64-element steps of x in flight, as shared memory allows (5 at least)
-constexpr int CODE_STAGES = 3;   // 256-element boxes of packed W in flight
+constexpr int CODE_STAGES = 4;   // 256-element boxes of packed W in flight; even: a warpgroup sees every use of its stages
+                                 // (a wait for a phase tells it from the one before alone)
 constexpr int PAIRS = 4;         // pairs of steps of decoded W in tensor memory, one for each warpgroup
 constexpr int SMEM = 231424;     // of a CTA, with barriers and alignment
 constexpr int CODE_BYTES = 128 * 128;
@@ -212,9 +213,10 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
       uint4 c[4];
 #pragma unroll
       for (int k = 0; k < 4; k++) c[k] = *reinterpret_cast<const uint4 *>(src + (((4 * (g & 1) + k) ^ (r & 7)) << 4));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty_w[cs]);
-      if (8 * t + 2 * g >= steps) break;   // behind the last step
+      if (8 * t + 2 * g >= steps) {   // behind the last step: nothing of the box is used
+        if (lane == 0) mbar_arrive(&empty_w[cs]);
+        break;
+      }
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         const uint32_t w[8] = {c[2 * u].x,     c[2 * u].y,     c[2 * u].z,     c[2 * u].w,
@@ -233,7 +235,12 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full_a[g]);
+      if (lane == 0) {
+        mbar_arrive(&full_a[g]);
+        // only here: the decoding has used every lane's words, so their loads are done (an arrival right behind
+        // the loads let the next box overwrite words that were still on their way)
+        mbar_arrive(&empty_w[cs]);
+      }
       m0 = n0;
       m1 = n1;
       n0 = o0;

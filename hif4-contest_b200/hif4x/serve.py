@@ -20,6 +20,7 @@ import torch
 from . import _lib as L
 
 GROUP = 64
+_I32 = (torch.int32,)
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 
@@ -140,15 +141,20 @@ class PagedKV:
     def __init__(self, k_codes: torch.Tensor, k_meta: torch.Tensor, v_codes: torch.Tensor, v_meta: torch.Tensor):
         _cuda(k_codes, "k_codes", (torch.uint8,), 4)
         dev = k_codes.device
-        n, h, p, half = k_codes.shape
-        for t, name, dt, last in ((k_meta, "k_meta", torch.int32, half // 32), (v_codes, "v_codes", torch.uint8, half),
-                                  (v_meta, "v_meta", torch.int32, half // 32)):
-            _cuda(t, name, (dt,), 4, dev)
-            if tuple(t.shape) != (n, h, p, last):
-                raise ValueError(f"{name} is {tuple(t.shape)}: {(n, h, p, last)} wanted")
-        for t in (k_codes, k_meta, v_codes, v_meta):
-            if not t.is_contiguous() or t.data_ptr() % 16:
-                raise ValueError("the cache's tensors must be contiguous and 16-byte aligned")
+        shape = k_codes.shape
+        n, h, p, half = shape
+        _cuda(k_meta, "k_meta", _I32, 4, dev)
+        _cuda(v_codes, "v_codes", (torch.uint8,), 4, dev)
+        _cuda(v_meta, "v_meta", _I32, 4, dev)
+        meta = torch.Size((n, h, p, half // 32))
+        if not (v_codes.shape == shape and k_meta.shape == meta and v_meta.shape == meta):
+            raise ValueError(f"v_codes {tuple(v_codes.shape)}, k_meta {tuple(k_meta.shape)} and v_meta "
+                             f"{tuple(v_meta.shape)} do not go with k_codes {tuple(shape)}: {tuple(shape)} and "
+                             f"{tuple(meta)} wanted")
+        at = [t.data_ptr() for t in (k_codes, k_meta, v_codes, v_meta)]
+        if (at[0] | at[1] | at[2] | at[3]) % 16 or not (k_codes.is_contiguous() and k_meta.is_contiguous()
+                                                        and v_codes.is_contiguous() and v_meta.is_contiguous()):
+            raise ValueError("the cache's tensors must be contiguous and 16-byte aligned")
         if half not in (32, 64):
             raise ValueError(f"head_dim {2 * half}: 64 or 128 wanted")
         if p not in (16, 32, 64, 128, 256):
@@ -157,8 +163,8 @@ class PagedKV:
             raise ValueError("the cache has no pages or no heads")
         self.k_codes, self.k_meta, self.v_codes, self.v_meta = k_codes, k_meta, v_codes, v_meta
         self.num_pages, self.kv_heads, self.page_size, self.head_dim, self.device = n, h, p, 2 * half, dev
-        self._desc = L.KVCacheDesc(k_codes.data_ptr(), k_meta.data_ptr(), v_codes.data_ptr(), v_meta.data_ptr(), n,
-                                   p, h, 2 * half)
+        self._desc = L.KVCacheDesc(*at, n, p, h, 2 * half)
+        self._ref = ctypes.byref(self._desc)
 
     @staticmethod
     def empty(num_pages: int, page_size: int, kv_heads: int, head_dim: int, device) -> "PagedKV":
@@ -171,19 +177,20 @@ class PagedKV:
                        make(head_dim // 2, torch.uint8), make(head_dim // 64, torch.int32))
 
     def _batch(self, cu_new: torch.Tensor, kv_len: torch.Tensor, pages: torch.Tensor) -> L.KVBatchDesc:
-        for t, name, dim in ((cu_new, "cu_new", 1), (kv_len, "kv_len", 1), (pages, "pages", 2)):
-            _cuda(t, name, (torch.int32,), dim, self.device)
-        B = kv_len.shape[0]
-        if B == 0 or cu_new.shape[0] != B + 1 or pages.shape[0] != B or pages.shape[1] == 0:
+        dev = self.device
+        _cuda(cu_new, "cu_new", _I32, 1, dev)
+        _cuda(kv_len, "kv_len", _I32, 1, dev)
+        _cuda(pages, "pages", _I32, 2, dev)
+        B, (rows, most) = kv_len.shape[0], pages.shape
+        if B == 0 or cu_new.shape[0] != B + 1 or rows != B or most == 0:
             raise ValueError(f"cu_new {tuple(cu_new.shape)}, kv_len {tuple(kv_len.shape)} and pages "
                              f"{tuple(pages.shape)} describe no batch: (B + 1,), (B,) and (B, most) wanted")
+        ld, unit = pages.stride()
         if cu_new.stride(0) != 1 or (B > 1 and kv_len.stride(0) != 1):
             raise ValueError("cu_new and kv_len must be contiguous")
-        most = pages.shape[1]
-        if (most > 1 and pages.stride(1) != 1) or (B > 1 and pages.stride(0) < most):
+        if (most > 1 and unit != 1) or (B > 1 and ld < most):
             raise ValueError("pages needs unit stride along its last dimension and rows apart")
-        return L.KVBatchDesc(cu_new.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), B, most,
-                             pages.stride(0) if B > 1 else most)
+        return L.KVBatchDesc(cu_new.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), B, most, ld if B > 1 else most)
 
 
 def _heads(t: torch.Tensor, name: str, dtypes, cache: PagedKV, heads: int | None = None):
@@ -220,7 +227,7 @@ def kv_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, cu_new: torch.Te
     batch = cache._batch(cu_new, kv_len, pages)
     if k.shape[0] == 0:
         return
-    _call(cache.device, "hif4x_kv_append", ctypes.byref(cache._desc), ctypes.byref(batch), k.data_ptr(), k.stride(0),
+    _call(cache.device, "hif4x_kv_append", cache._ref, ctypes.byref(batch), k.data_ptr(), k.stride(0),
           k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), L.dtype_code(k.dtype), k.shape[0])
 
 
@@ -245,7 +252,7 @@ def kv_read(cache: PagedKV, cu_new: torch.Tensor, kv_len: torch.Tensor, pages: t
         if rows and (k.data_ptr() % 16 or v.data_ptr() % 16 or _overlap(k, v)):
             raise ValueError("out must be two 16-byte aligned tensors apart")
     if rows:
-        _call(cache.device, "hif4x_kv_read", ctypes.byref(cache._desc), ctypes.byref(batch), rows, k.data_ptr(),
+        _call(cache.device, "hif4x_kv_read", cache._ref, ctypes.byref(batch), rows, k.data_ptr(),
               v.data_ptr(), L.dtype_code(k.dtype))
     return k, v
 
@@ -298,7 +305,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, cu_new: torch.Tensor, kv_le
     need = _attention_work(cache.device, cache.page_size, cache.kv_heads, dh, batch.sequences, batch.max_pages, heads,
                            rows, window, sinks, most)
     work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
-    _call(cache.device, "hif4x_paged_attention", ctypes.byref(cache._desc), ctypes.byref(batch), q.data_ptr(), qr, qh,
+    _call(cache.device, "hif4x_paged_attention", cache._ref, ctypes.byref(batch), q.data_ptr(), qr, qh,
           heads, rows, dh ** -0.5 if scale is None else float(scale), window, sinks, most, out.data_ptr(), orow, ohead,
           None if work is None else work.data_ptr(), need)
     return out

@@ -146,6 +146,18 @@ def test_linear_special_values():
         check_linear(x, meta, codes, y, act=act)
 
 
+@pytest.mark.parametrize("T,N,C,runs", [(1, 1000, 14336, 300), (64, 4096, 14336, 100), (300, 1000, 2048, 100),
+                                        (2048, 2048, 4096, 30)])
+def test_linear_is_reproducible(T, N, C, runs):
+    """Every call gives the same bits (a box of codes or a stage reused too early shows here)."""
+    meta, codes = packed(31, N, C, scale=0.02)
+    x = torch.randn(T, C, generator=gen(C), device="cuda").bfloat16()
+    first = serve.linear(x, meta, codes)
+    check_linear(x, meta, codes, first)
+    same = [torch.equal(serve.linear(x, meta, codes), first) for _ in range(runs)]
+    assert all(same), f"{same.count(False)} of {runs} runs differ"
+
+
 # ------------------------------------------------------------------ the cache
 class Batch:
     """A cache with ragged sequences: random pages in random order, `spare` pages that are nobody's."""
@@ -338,9 +350,10 @@ def test_attention(new, lens, qh, kvh, dh, page, window, sinks):
 def test_attention_is_reproducible():
     b = Batch([1] * 5 + [70], [900, 3, 4000, 64, 65, 2000], 2, 128, 64, 1)
     q = torch.randn(b.rows, 8, 128, generator=gen(1), device="cuda").bfloat16()
-    first = serve.paged_attention(q, b.cache, *b.args)
-    for _ in range(5):
-        assert torch.equal(first, serve.paged_attention(q, b.cache, *b.args))
+    for kw in ({}, {"window": 300, "sinks": 70}, {"max_new": 1}):
+        first = serve.paged_attention(q, b.cache, *b.args, **kw)
+        same = [torch.equal(first, serve.paged_attention(q, b.cache, *b.args, **kw)) for _ in range(200)]
+        assert all(same), f"{same.count(False)} runs differ"
 
 
 @pytest.mark.parametrize("new", [[2, 1], [60, 100]])
