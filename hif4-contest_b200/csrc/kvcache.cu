@@ -219,10 +219,18 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendArgs p) {
   uint32_t meta = ((lv & 1u) << (8 + sub)) | ((lv >> 1) << (16 + 2 * sub));
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) meta |= __shfl_xor_sync(mask, meta, o);
+  // m = min(RNE(|x| / unit * 4), 7) as the codec's packed form computes it: the quotient by sf after Markstein
+  // (exact for E6M2 significands), rescaled by the lv factors, clamped at 7.25 and rounded by the magic number
+  const float ysf = __fdiv_rn(1.0f, sf);
+  const u64 YSF2 = pk2(ysf, ysf), NSF2 = pk2(-sf, -sf), MAG2 = pk2(kMagic, kMagic);
 #pragma unroll
-  for (int k = 0; k < 8; k++) {
-    const uint32_t l = (lv & 1u) + ((lv >> (1 + k / 4)) & 1u);
-    nib |= (uint32_t)mant4_ref(a[k], __fmul_rn(sf, l == 0 ? 1.0f : l == 1 ? 2.0f : 4.0f)) << (4 * k);
+  for (int k = 0; k < 8; k += 2) {
+    const float mq = exp2i(2 - (int)((lv & 1u) + ((lv >> (1 + k / 4)) & 1u)));
+    const u64 a2 = pk2(a[k], a[k + 1]), q0 = mul2(a2, YSF2);
+    float lo, hi;
+    upk2(mul2(fma2(fma2(q0, NSF2, a2), YSF2, q0), pk2(mq, mq)), lo, hi);
+    upk2(add2(pk2(fminf(lo, 7.25f), fminf(hi, 7.25f)), MAG2), lo, hi);
+    nib |= ((__float_as_uint(lo) & 7u) | ((__float_as_uint(hi) & 7u) << 4)) << (4 * k);
   }
   const int64_t unit = row * c.nb + gi;
   reinterpret_cast<uint32_t *>(c.codes[which])[unit * 8 + sub] = nib;
@@ -235,32 +243,35 @@ struct ReadArgs {
   int dtype;
 };
 
-// Rows back out: the thread of (token, head, sub-block) writes eight values.
+// Rows back out: eight lanes have a (token, head), lane i sub-block i of its
+// 64-groups of K and V; the place is looked up once for all of them.
 __global__ void __launch_bounds__(128) read_kernel(const ReadArgs p) {
   const CacheArgs &c = p.c;
   const int lane = threadIdx.x & 31, sub = lane & 7;
-  const int64_t per = (int64_t)c.heads * c.nb;
-  const int64_t g = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
-  if (g >= c.rows * per) return;
-  const int which = blockIdx.y;
-  const int64_t token = g / per;
-  const int r = (int)(g - token * per), head = r / c.nb, gi = r - head * c.nb;
-  const int64_t row = cache_row(c, token, head, sub, 0xffu << (lane & 24));
+  const int64_t g = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;   // (token, head)
+  if (g >= c.rows * c.heads) return;
+  const int64_t token = g / c.heads;
+  const int64_t row = cache_row(c, token, (int)(g - token * c.heads), sub, 0xffu << (lane & 24));
   if (row < 0) return;
-  const int64_t unit = row * c.nb + gi;
-  const uint32_t w = reinterpret_cast<const uint32_t *>(c.codes[which])[unit * 8 + sub];
-  const uint32_t m = c.meta[which][unit];
-  uint32_t o[4];
-  hif4_decode8<0>(w, Hif4Levels(m, sub), hif4_sf2(m), o);
-  const int64_t at = g * 8 + sub;
-  if (p.dtype == HIF4X_DT_BF16) {
-    static_cast<uint4 *>(p.out[which])[at] = make_uint4(o[0], o[1], o[2], o[3]);
-  } else {
-    float4 *d = static_cast<float4 *>(p.out[which]) + 2 * at;
-    d[0] = make_float4(__uint_as_float(o[0] << 16), __uint_as_float(o[0] & 0xffff0000u), __uint_as_float(o[1] << 16),
-                       __uint_as_float(o[1] & 0xffff0000u));
-    d[1] = make_float4(__uint_as_float(o[2] << 16), __uint_as_float(o[2] & 0xffff0000u), __uint_as_float(o[3] << 16),
-                       __uint_as_float(o[3] & 0xffff0000u));
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    const int which = u & 1, gi = u >> 1;
+    if (gi >= c.nb) break;
+    const int64_t unit = row * c.nb + gi;
+    const uint32_t w = reinterpret_cast<const uint32_t *>(c.codes[which])[unit * 8 + sub];
+    const uint32_t m = c.meta[which][unit];
+    uint32_t o[4];
+    hif4_decode8<0>(w, Hif4Levels(m, sub), hif4_sf2(m), o);
+    const int64_t at = (g * c.nb + gi) * 8 + sub;
+    if (p.dtype == HIF4X_DT_BF16) {
+      static_cast<uint4 *>(p.out[which])[at] = make_uint4(o[0], o[1], o[2], o[3]);
+    } else {
+      float4 *d = static_cast<float4 *>(p.out[which]) + 2 * at;
+      d[0] = make_float4(__uint_as_float(o[0] << 16), __uint_as_float(o[0] & 0xffff0000u),
+                         __uint_as_float(o[1] << 16), __uint_as_float(o[1] & 0xffff0000u));
+      d[1] = make_float4(__uint_as_float(o[2] << 16), __uint_as_float(o[2] & 0xffff0000u),
+                         __uint_as_float(o[3] << 16), __uint_as_float(o[3] & 0xffff0000u));
+    }
   }
 }
 
@@ -299,10 +310,11 @@ int cache_args(const hif4x_kv_cache *kv, const hif4x_kv_batch *b, int64_t rows, 
   return a->status ? HIF4X_OK : HIF4X_ERR_LAUNCH;
 }
 
-static int grid_of(const CacheArgs &a, dim3 *grid) {
-  const int64_t blocks = (a.rows * a.heads * a.nb * 8 + 127) / 128;
+// Eight lanes for each of `groups` (row, head, ...), in CTAs of 128; K and V as y where `y` is 2.
+static int grid_of(int64_t groups, unsigned y, dim3 *grid) {
+  const int64_t blocks = (groups * 8 + 127) / 128;
   if (blocks > INT32_MAX) return HIF4X_ERR_UNSUPPORTED;
-  *grid = dim3((unsigned)blocks, 2);
+  *grid = dim3((unsigned)blocks, y);
   return HIF4X_OK;
 }
 
@@ -329,7 +341,7 @@ extern "C" int hif4x_kv_append(const hif4x_kv_cache *kv, const hif4x_kv_batch *b
   p.vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 && k_ld_row % unit == 0 &&
           k_ld_head % unit == 0 && v_ld_row % unit == 0 && v_ld_head % unit == 0;
   dim3 grid;
-  st = grid_of(p.c, &grid);
+  st = grid_of(rows * p.c.heads * p.c.nb, 2, &grid);
   if (st != HIF4X_OK) return st;
   append_kernel<<<grid, 128, 0, (cudaStream_t)stream>>>(p);
   HIF4X_CHECK_LAUNCH();
@@ -348,7 +360,7 @@ extern "C" int hif4x_kv_read(const hif4x_kv_cache *kv, const hif4x_kv_batch *bat
   p.out[1] = v;
   p.dtype = dtype;
   dim3 grid;
-  st = grid_of(p.c, &grid);
+  st = grid_of(rows * p.c.heads, 1, &grid);
   if (st != HIF4X_OK) return st;
   read_kernel<<<grid, 128, 0, (cudaStream_t)stream>>>(p);
   HIF4X_CHECK_LAUNCH();

@@ -17,7 +17,7 @@
 //            32 columns of bf16 pairs to tensor memory, where the MMA reads A
 //            from.  (A decoding warp alone issues an instruction in 5 to 6
 //            cycles: with two warps a scheduler a step took 830 cycles, with
-//            four 600, of which the ALU pipe is busy for 330.)  W's tile never passes shared memory as bf16: that leaves
+//            four XXXX; the ALU pipe's floor is 270.)  W's tile never passes shared memory as bf16: that leaves
 //            shared memory's bandwidth to x alone (a 128 x 256 x 64 step would
 //            otherwise write and read 96 KB there, more than its MMA time).
 // C is shared out over a cluster of up to 4 CTAs where the tiles alone do not
@@ -36,11 +36,8 @@ namespace lin {
 
 using namespace tc;
 
-constexpr int MOST_X = 8;        // 64-element steps of x in flight, as shared memory allows (5 at least)
-constexpr int CODE_STAGES = 4;   // 256-element boxes of packed W in flight; even: a warpgroup sees every use of its stages
-                                 // (a wait for a phase tells it from the one before alone)
-constexpr int PAIRS = 4;         // pairs of steps of decoded W in tensor memory, one for each warpgroup
-constexpr int SMEM = 231424;     // of a CTA, with barriers and alignment
+constexpr int STAGES = 4;        // 64-element steps of x and of decoded W in flight
+constexpr int CODE_STAGES = 3;   // 256-element boxes of packed W in flight
 constexpr int CODE_BYTES = 128 * 128;
 constexpr int THREADS = 640;
 constexpr int BM = 128;
@@ -57,7 +54,7 @@ struct Args {
   uint16_t *y;
   int64_t ldy;
   int vec;                  // rows of y and residual take 16-byte accesses
-  int xs;                   // stages of x
+  uint32_t tmem_cols;
   int *status;
 };
 
@@ -97,10 +94,10 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int x_bytes = a.nt * 128;
-  uint8_t *sx = smem, *sw = smem + a.xs * x_bytes;
-  uint64_t *full_x = reinterpret_cast<uint64_t *>(sw + CODE_STAGES * CODE_BYTES), *empty_x = full_x + MOST_X;
-  uint64_t *full_a = empty_x + MOST_X, *empty_a = full_a + PAIRS;
-  uint64_t *full_w = empty_a + PAIRS, *empty_w = full_w + CODE_STAGES, *done = empty_w + CODE_STAGES;
+  uint8_t *sx = smem, *sw = smem + STAGES * x_bytes;
+  uint64_t *full_x = reinterpret_cast<uint64_t *>(sw + CODE_STAGES * CODE_BYTES);
+  uint64_t *full_a = full_x + STAGES, *empty = full_a + STAGES, *full_w = empty + STAGES;
+  uint64_t *empty_w = full_w + CODE_STAGES, *done = empty_w + CODE_STAGES;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -109,17 +106,14 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
   const int k0 = min(a.nb, rank * a.per), steps = min(a.nb, k0 + a.per) - k0;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < a.xs; s++) {
+    for (int s = 0; s < STAGES; s++) {
       mbar_init(&full_x[s], 1);
-      mbar_init(&empty_x[s], 1);
-    }
-    for (int s = 0; s < PAIRS; s++) {
       mbar_init(&full_a[s], 4);
-      mbar_init(&empty_a[s], 1);
+      mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < CODE_STAGES; s++) {
       mbar_init(&full_w[s], 1);
-      mbar_init(&empty_w[s], 8);
+      mbar_init(&empty_w[s], 16);
     }
     mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -127,54 +121,44 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
   if (warp == 1) {
     __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(512));
+                 "r"(a.tmem_cols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_a = *tmem_slot, tmem_d = tmem_a + PAIRS * 64;   // decoded W, then the accumulator (256 columns)
+  const uint32_t tmem_a = *tmem_slot, tmem_d = tmem_a + STAGES * 32;   // A stages, then the accumulator
   bool ok = true;
 
   if (warp == 0) {
     if (elect_one()) {
-      int i = 0, s = 0, ph = 1;
+      int i = 0;
       for (; i < steps; i++) {
-        if (i >= a.xs) ok = mbar_wait_sleep(&empty_x[s], ph, a.status);
+        const int s = i % STAGES;
+        if (i >= STAGES) ok = mbar_wait_sleep(&empty[s], ((i / STAGES) - 1) & 1, a.status);
         if (!ok) break;
         mbar_expect_tx(&full_x[s], x_bytes);
         tma_load_2d(&map_x, sx + s * x_bytes, &full_x[s], (k0 + i) * 64, (int)tok0);
-        if (++s == a.xs) {
-          s = 0;
-          ph ^= 1;
-        }
       }
       // no copy may be in flight when the CTA ends
-      for (int k = max(0, i - a.xs); k < i; k++) mbar_wait_sleep(&full_x[k % a.xs], (k / a.xs) & 1, a.status);
+      for (int s = 0; s < STAGES; s++)
+        if (i > s) mbar_wait_sleep(&full_x[s], ((i - 1 - s) / STAGES) & 1, a.status);
     }
   } else if (warp == 1) {
     if (elect_one()) {
       const uint32_t idesc = idesc_bf16((uint32_t)a.nt, 0);
       const uint64_t dx = smem_desc(smem_u32(sx), 16u, 1024u, 2u);   // + 2 for 32 bytes further
-      int s = 0, ph = 0;
-      for (int i = 0; i < steps && ok; i += 2) {   // a warpgroup's pair of steps
-        const int g = (i >> 1) & 3;
-        ok = mbar_wait_sleep(&full_a[g], (i >> 3) & 1, a.status);
-        for (int u = i; u < min(i + 2, steps) && ok; u++) {
-          ok = mbar_wait_sleep(&full_x[s], ph, a.status);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t x = dx + (uint32_t)(s * x_bytes >> 4);
+      for (int i = 0; i < steps; i++) {
+        const int s = i % STAGES, ph = (i / STAGES) & 1;
+        ok = mbar_wait_sleep(&full_x[s], ph, a.status) &&
+             mbar_wait_sleep(&full_a[s], ph, a.status);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t x = dx + (uint32_t)(s * x_bytes >> 4);
 #pragma unroll
-          for (int j = 0; j < 4; j++)
-            mma_f16_ts(tmem_d, tmem_a + g * 64 + (u & 1) * 32 + j * 8, x + 2 * j, idesc, (u > 0 || j > 0) ? 1u : 0u);
-          mma_commit(&empty_x[s]);
-          if (++s == a.xs) {
-            s = 0;
-            ph ^= 1;
-          }
-        }
-        mma_commit(&empty_a[g]);
+        for (int j = 0; j < 4; j++)
+          mma_f16_ts(tmem_d, tmem_a + s * 32 + j * 8, x + 2 * j, idesc, (i > 0 || j > 0) ? 1u : 0u);
+        mma_commit(&empty[s]);
       }
       mma_commit(done);
     }
@@ -193,58 +177,48 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
         if (i > s) mbar_wait_sleep(&full_w[s], ((i - 1 - s) / CODE_STAGES) & 1, a.status);
     }
   } else if (warp >= 4) {
-    // ---- decode: thread = row of W (tensor memory lane); of every eight steps warpgroup g has 2 g and 2 g + 1,
-    // the half g & 1 of every other box
+    // ---- decode: thread = row of W (tensor memory lane); warpgroup g has group g of every box, stage g
     const int g = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
     const int64_t row = row0 + r;
-    const uint32_t *meta = a.meta + (row < a.N ? row : 0) * a.nb + k0 + 2 * g;
+    const uint32_t *meta = a.meta + (row < a.N ? row : 0) * a.nb + k0 + g;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const int boxes = (steps + 3) / 4;
-    auto meta_of = [&](int t, int u) { return 8 * t + 2 * g + u < steps ? __ldg(meta + 8 * t + u) : 0u; };
-    uint32_t m0 = meta_of(0, 0), m1 = meta_of(0, 1), n0 = meta_of(1, 0), n1 = meta_of(1, 1);
-    for (int t = 0, b = g >> 1; b < boxes; t++, b += 2) {
-      const uint32_t o0 = meta_of(t + 2, 0), o1 = meta_of(t + 2, 1);
-      const int cs = b % CODE_STAGES;
-      ok = mbar_wait_sleep(&full_w[cs], (b / CODE_STAGES) & 1, a.status);
+    // 16-byte chunk c of row r lies at chunk c ^ (r & 7)
+    const uint8_t *src0 = sw + r * 128 + (((2 * g) ^ (r & 7)) << 4), *src1 = sw + r * 128 + (((2 * g + 1) ^ (r & 7)) << 4);
+    const int boxes = (steps + 3) / 4, mine = (steps - g + 3) / 4;   // this warpgroup's steps: the first boxes
+    uint32_t m = mine > 0 ? __ldg(meta) : 0u;
+    int cs = 0, cp = 0;   // code stage and its phase
+    for (int b = 0; b < boxes && ok; b++) {
+      const uint32_t next = b + 1 < mine ? __ldg(meta + 4 * (b + 1)) : 0u;
+      ok = mbar_wait_sleep(&full_w[cs], cp, a.status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      // 16-byte chunk c of row r lies at chunk c ^ (r & 7)
-      const uint8_t *src = sw + cs * CODE_BYTES + r * 128;
-      uint4 c[4];
-#pragma unroll
-      for (int k = 0; k < 4; k++) c[k] = *reinterpret_cast<const uint4 *>(src + (((4 * (g & 1) + k) ^ (r & 7)) << 4));
-      if (8 * t + 2 * g >= steps) {   // behind the last step: nothing of the box is used
-        if (lane == 0) mbar_arrive(&empty_w[cs]);
-        break;
-      }
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const uint32_t w[8] = {c[2 * u].x,     c[2 * u].y,     c[2 * u].z,     c[2 * u].w,
-                               c[2 * u + 1].x, c[2 * u + 1].y, c[2 * u + 1].z, c[2 * u + 1].w};
+      const uint4 c0 = *reinterpret_cast<const uint4 *>(src0 + cs * CODE_BYTES);
+      const uint4 c1 = *reinterpret_cast<const uint4 *>(src1 + cs * CODE_BYTES);
+      if (b < mine) {
+        const uint32_t w[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
         uint32_t v[32];
-        hif4_decode64(w, u ? m1 : m0, v);
-        if (u == 0 && t > 0) {
-          ok = mbar_wait_sleep(&empty_a[g], (t - 1) & 1, a.status);
+        hif4_decode64(w, m, v);
+        if (b > 0) {
+          ok = mbar_wait_sleep(&empty[g], (b - 1) & 1, a.status);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
         }
-        tmem_st32(tmem_a + lanes + g * 64 + u * 32, v);
+        tmem_st32(tmem_a + lanes + g * 32, v);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full_a[g]);
       }
-      if (!ok) break;
-      tmem_wait_st();
-      tc_fence_before();
+      // the box is given back here, where the decoding has used every lane's words: behind their loads alone, the
+      // next box could overwrite words still on their way
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&full_a[g]);
-        // only here: the decoding has used every lane's words, so their loads are done (an arrival right behind
-        // the loads let the next box overwrite words that were still on their way)
-        mbar_arrive(&empty_w[cs]);
+      if (lane == 0) mbar_arrive(&empty_w[cs]);
+      if (++cs == CODE_STAGES) {
+        cs = 0;
+        cp ^= 1;
       }
-      m0 = n0;
-      m1 = n1;
-      n0 = o0;
-      n1 = o1;
+      m = next;
     }
     // ---- the accumulator to shared memory, [x row][row of W], over the x stages
     ok = mbar_wait_sleep(done, 0, a.status);
@@ -269,7 +243,7 @@ __global__ void __launch_bounds__(THREADS) linear_kernel(const __grid_constant__
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_a), "r"(512));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_a), "r"(a.tmem_cols));
   }
   if (ranks > 1) cluster_sync();
   // ---- the ranks' sums, bias, activation, residual: 8 outputs of one x row a thread
@@ -354,6 +328,10 @@ static bool map_rows(CUtensorMap *map, CUtensorMapDataType type, const void *bas
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+static int smem_bytes(int nt) {
+  return STAGES * nt * 128 + CODE_STAGES * CODE_BYTES + (3 * STAGES + 2 * CODE_STAGES + 1) * 8 + 16 + 1024;
+}
+
 }  // namespace lin
 }  // namespace hif4x
 
@@ -376,7 +354,7 @@ extern "C" int hif4x_linear_packed(const void *x, int64_t ldx, const uint32_t *m
   static std::once_flag once[kMaxDevices];
   static bool attr_ok[kMaxDevices];
   std::call_once(once[dev], [dev] {
-    attr_ok[dev] = cudaFuncSetAttribute(linear_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) ==
+    attr_ok[dev] = cudaFuncSetAttribute(linear_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(256)) ==
                    cudaSuccess;
   });
   Args a{};
@@ -418,7 +396,7 @@ extern "C" int hif4x_linear_packed(const void *x, int64_t ldx, const uint32_t *m
   a.ldy = ldy;
   a.vec = (reinterpret_cast<uintptr_t>(y) & 15u) == 0 && ldy % 8 == 0 &&
           (!residual || ((reinterpret_cast<uintptr_t>(residual) & 15u) == 0 && ldr % 8 == 0));
-  a.xs = std::min(MOST_X, (SMEM - 1024 - 512 - CODE_STAGES * CODE_BYTES) / (a.nt * 128));
+  a.tmem_cols = a.nt <= 128 ? 256u : 512u;
   CUtensorMap mx, mw;
   if (!map_rows(&mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, C, T, ldx * 2, 64, a.nt) ||
       !map_rows(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, C / 2, N, C / 2, 128, BM))
@@ -426,7 +404,7 @@ extern "C" int hif4x_linear_packed(const void *x, int64_t ldx, const uint32_t *m
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)tiles_n, (unsigned)tiles_t, (unsigned)ranks);
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = a.xs * a.nt * 128 + CODE_STAGES * CODE_BYTES + 512 + 1024;
+  cfg.dynamicSmemBytes = smem_bytes(a.nt);
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
