@@ -959,12 +959,13 @@ __global__ void __launch_bounds__(128) attend_join_kernel(const AttendArgs a) {
 // second wave would leave most of them idle; 65536 keys of one sequence: 50
 // us, 91 with three waves).  Many: twelve CTAs for every SM, so that sequences
 // of several lengths even out (64 sequences of up to 8192 keys: 180 us, 289
-// unshared).  No share under two tiles for each warp, and no more than 2^26
-// partial sums (256 MB) in all.
+// unshared).  No share under 512 keys (eight tiles for each warp; the join is
+// a launch of its own, 4 us), and no more than 2^26 partial sums (256 MB) in
+// all.
 static int attend_splits(int sms, int64_t lanes, int64_t keys, int64_t outputs, bool two) {
   const int64_t at_once = (two ? 2 : 3) * (int64_t)sms;
   const int64_t want = lanes * 4 <= at_once * 3 ? at_once / lanes : (12 * (int64_t)sms + lanes - 1) / lanes;
-  const int64_t most = std::max<int64_t>(1, keys / (16 * 4 * 2));
+  const int64_t most = std::max<int64_t>(1, keys / 512);
   const int64_t room = (int64_t(1) << 26) / std::max<int64_t>(1, outputs);
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, room, MOST_SPLITS}));
 }
