@@ -645,6 +645,7 @@ int device_sms(int dev) {
   static std::once_flag once[kMaxDevices];
   if (dev < 0 || dev >= kMaxDevices) return 0;
   std::call_once(once[dev], [dev] {
+    RelaxedCapture relaxed;
     int n = 0;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) n = 0;
     cudaMemPool_t pool;
@@ -752,15 +753,19 @@ int gemm_split(const float *As, int a_products, const float *Bs, int b_products,
   return cudaGetLastError() == cudaSuccess ? HIF4X_OK : HIF4X_ERR_LAUNCH;
 }
 
-// Device address of the sticky status word on device `dev` (the current one), looked up once; null on failure.
+// Device address of the sticky status word on device `dev` (the current one),
+// looked up once; null on failure, which the next call tries again.
 int *status_word(int dev) {
+  static std::mutex lock;
   static int *word[kMaxDevices];
-  static std::once_flag once[kMaxDevices];
   if (dev < 0 || dev >= kMaxDevices) return nullptr;
-  std::call_once(once[dev], [dev] {
+  std::lock_guard<std::mutex> hold(lock);
+  if (word[dev] == nullptr) {
+    RelaxedCapture relaxed;
     void *p = nullptr;
-    word[dev] = cudaGetSymbolAddress(&p, g_status) == cudaSuccess ? static_cast<int *>(p) : nullptr;
-  });
+    if (cudaGetSymbolAddress(&p, g_status) == cudaSuccess) word[dev] = static_cast<int *>(p);
+    else cudaGetLastError();
+  }
   return word[dev];
 }
 

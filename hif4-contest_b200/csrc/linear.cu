@@ -351,15 +351,10 @@ extern "C" int hif4x_linear_packed(const void *x, int64_t ldx, const uint32_t *m
   if (cudaGetDevice(&dev) != cudaSuccess) return HIF4X_ERR_LAUNCH;
   const int sms = device_sms(dev);
   if (sms <= 0 || dev >= kMaxDevices) return HIF4X_ERR_LAUNCH;
-  static std::once_flag once[kMaxDevices];
-  static bool attr_ok[kMaxDevices];
-  std::call_once(once[dev], [dev] {
-    attr_ok[dev] = cudaFuncSetAttribute(linear_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(256)) ==
-                   cudaSuccess;
-  });
+  static SharedOptIn opt_in;
   Args a{};
   a.status = status_word(dev);
-  if (!attr_ok[dev] || !a.status) return HIF4X_ERR_LAUNCH;
+  if (!opt_in(linear_kernel, smem_bytes(256), dev) || !a.status) return HIF4X_ERR_LAUNCH;
 
   const int64_t tiles_n = (N + BM - 1) / BM;
   // x rows of a tile, all tiles alike: of the tilings from the fewest tiles on, the one whose waves of CTAs take

@@ -169,8 +169,8 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) attend_rows_kernel(const
   const int64_t room = (int64_t)c.most << c.page_shift;
   const int old = c.kv_len[s] - n_new;   // position of the first new row
   const int *pages = c.pages + s * c.ld_pages;
-  const int64_t rows = (int64_t)n_new * a.group;
-  if (rows > a.most_rows) return;
+  if (cu0 < 0 || cu0 >= c.rows || (int64_t)n_new * a.group > a.most_rows) return;
+  const int64_t rows = min((int64_t)n_new, c.rows - cu0) * a.group;   // rows that the batch's tensors do not have: none
 
   for (int64_t r0 = 0; r0 < rows; r0 += ROWS) {
     const int64_t r1 = min(rows, r0 + ROWS);
@@ -1020,14 +1020,8 @@ static int attend_plan(const AttendSizes &z, AttendPlan *p) {
 
 template <int DH>
 static int launch_tiles(AttendArgs a, int dev, const AttendPlan &p, cudaStream_t s) {
-  static std::once_flag once[tc::kMaxDevices];
-  static bool attr_ok[tc::kMaxDevices];
-  if (dev < 0 || dev >= tc::kMaxDevices) return HIF4X_ERR_LAUNCH;
-  std::call_once(once[dev], [dev] {
-    attr_ok[dev] = cudaFuncSetAttribute(tiles::attend_tiles_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        tiles::Cfg<DH>::SMEM) == cudaSuccess;
-  });
-  if (!attr_ok[dev]) return HIF4X_ERR_LAUNCH;
+  static tc::SharedOptIn opt_in;
+  if (!opt_in(tiles::attend_tiles_kernel<DH>, tiles::Cfg<DH>::SMEM, dev)) return HIF4X_ERR_LAUNCH;
   // the kernel compares unscaled scores, so its scale is positive: a negative one turns the queries' signs
   const int flip = a.scale < 0.0f;
   a.scale = std::max(std::fabs(a.scale), 1e-35f);

@@ -185,6 +185,31 @@ __device__ __forceinline__ void bulk_wait_read_1() { asm volatile("cp.async.bulk
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // ------------------------------------------------------------------ host
+// While it lives, this thread may make calls that a stream's capture forbids
+// otherwise (the lookups of a first call: none of them enqueues work).
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+// Dynamic shared memory opt-in of a kernel, a property of it in each device's
+// context: once per device; a failure is tried again by the next call.
+struct SharedOptIn {
+  std::mutex lock;
+  bool done[kMaxDevices] = {};
+  template <typename Kernel>
+  bool operator()(Kernel kernel, int bytes, int dev) {
+    if (dev < 0 || dev >= kMaxDevices) return false;
+    std::lock_guard<std::mutex> hold(lock);
+    if (!done[dev]) {
+      RelaxedCapture relaxed;
+      done[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+    }
+    return done[dev];
+  }
+};
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

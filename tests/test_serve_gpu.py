@@ -7,6 +7,9 @@ Tolerances are the roundings counted: one rounding to bf16 is off by at most
 cores truncate), summed over the magnitudes that enter.
 """
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -302,7 +305,7 @@ def check_attention(b, q, out, window=0, sinks=0, scale=None):
             got = out[at:at + n, h].double()
             # scores: dh + 4 fp32 steps of the magnitudes; a weight carries that error (and a few steps of
             # exp2 and of its sum) and one rounding to bf16; the result one more
-            err = (b.dh + 4) * F32 * scale * (qq.abs() @ kk.abs().t()).masked_fill(~see, 0).amax(1, keepdim=True) \
+            err = (b.dh + 4) * F32 * abs(scale) * (qq.abs() @ kk.abs().t()).masked_fill(~see, 0).amax(1, keepdim=True) \
                 if t.numel() else torch.zeros(n, 1, device="cuda").double()
             # scores are rounded once more in log2 units, relative to their size
             size = s.masked_fill(~see, 0).abs().amax(1, keepdim=True) if t.numel() else err
@@ -371,7 +374,7 @@ def test_attention_views_and_padding(new):
     assert (view[T:] == 5).all() and (out[:, :, 64:] == 5).all()
 
 
-@pytest.mark.parametrize("scale", [0.0, 1e-3, 1.0, 4.0])
+@pytest.mark.parametrize("scale", [-1.0, 0.0, 1e-3, 1.0, 4.0])
 @pytest.mark.parametrize("n", [1, 90])
 def test_attention_scales_and_peaks(scale, n):
     """Flat to peaked softmax, falling and rising scores (the running reference moves)."""
@@ -433,6 +436,35 @@ def test_attention_bad_pages(n):
     serve.paged_attention(q, b.cache, b.cu, b.len, short, max_new=n)
     with pytest.raises(L.Hif4xError, match="page"):
         linalg.check_device_status()
+
+
+def test_cache_beyond_32_bits():
+    """Pages more than 2^32 bytes into the codes, 2^31 into the meta words' bytes and on."""
+    pages, kvh, page, dh = 40000, 8, 256, 128
+    make = lambda last, dt: torch.empty(pages, kvh, page, last, dtype=dt, device="cuda")  # noqa: E731
+    cache = serve.PagedKV(make(64, torch.uint8), make(2, torch.int32), make(64, torch.uint8), make(2, torch.int32))
+    assert cache.k_codes.numel() > 2 ** 32
+    table = torch.tensor([[39999, 0, 33333], [32768, 39998, 16384]], dtype=torch.int32, device="cuda")
+    lens = [700, 520]
+    k, v = (torch.randn(sum(lens), kvh, dh, generator=gen(s), device="cuda").bfloat16() for s in (1, 2))
+    cu = torch.tensor([0, 700, 1220], dtype=torch.int32, device="cuda")
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    serve.kv_append(cache, k, v, cu, ln, table)
+    rk, rv = serve.kv_read(cache, cu, ln, table, rows=1220)
+    for got, src in ((rk, k), (rv, v)):
+        deq = codec.convert(src.float().reshape(-1, dh).contiguous(), kind=L.SRC_VALUES, dict5=False,
+                            deq_dtype=torch.float32)["deq"].view(src.shape)
+        assert torch.equal(got.float(), deq)
+    # the same rows in a small cache give the same attention, for both kernels
+    small = serve.PagedKV.empty(6, page, kvh, dh, "cuda")
+    near = torch.tensor([[3, 1, 0], [5, 2, 4]], dtype=torch.int32, device="cuda")
+    serve.kv_append(small, k, v, cu, ln, near)
+    for new in (1, 50):
+        q = torch.randn(2 * new, 32, dh, generator=gen(3), device="cuda").bfloat16()
+        c = torch.tensor([0, new, 2 * new], dtype=torch.int32, device="cuda")
+        assert torch.equal(serve.paged_attention(q, cache, c, ln, table, max_new=new),
+                           serve.paged_attention(q, small, c, ln, near, max_new=new))
+    linalg.check_device_status()
 
 
 # ------------------------------------------------------------------ together
@@ -514,6 +546,37 @@ def test_two_graphs_and_two_streams():
         o1.zero_(), o2.zero_()
         g1.replay(), g2.replay()
         assert torch.equal(o1, wb) and torch.equal(o2, wc)
+
+
+FIRST_CALL = """
+import sys; sys.path.insert(0, sys.argv[1])
+import torch
+from hif4x import serve
+x = torch.ones(3, 128, dtype=torch.bfloat16, device="cuda")
+meta, codes = torch.full((64, 2), 0xc0, dtype=torch.int32, device="cuda"), torch.full((64, 64), 0x44, dtype=torch.uint8, device="cuda")
+cache = serve.PagedKV.empty(4, 16, 1, 64, "cuda")
+cu, ln = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([0, 3], [3]))
+pages = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+long = torch.randn(60, 4, 64, device="cuda").bfloat16()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = serve.linear(x, meta, codes)
+    serve.kv_append(cache, y.view(3, 1, 64), y.view(3, 1, 64), cu, ln, pages)
+    o = serve.paged_attention(y.view(3, 1, 64), cache, cu, ln, pages, max_new=3)
+    serve.paged_attention(long, cache, cu * 20, ln, pages)
+for _ in range(2):
+    g.replay()
+torch.cuda.synchronize()
+assert (y == 128).all() and (o == 128).all(), (y, o)
+print("ok")
+"""
+
+
+def test_first_call_of_a_process_in_a_capture():
+    """Nothing that a call does the first time only is forbidden while a stream is captured."""
+    here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hif4-contest_b200")
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL, here], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "ok" in r.stdout, r.stderr[-2000:]
 
 
 # ------------------------------------------------------------------ refusals
