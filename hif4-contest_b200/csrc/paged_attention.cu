@@ -559,12 +559,12 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
   uint8_t *hidden = reinterpret_cast<uint8_t *>(found + 3);     // [4 steps][8 blocks of 16 keys]: 1 without a page
   const CacheArgs &c = a.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kh = blockIdx.y, split = blockIdx.z;
+  const int kh = blockIdx.x % c.heads, split = blockIdx.y;
 
-  // ---- which sequence and tile: the tiles of all sequences counted off, the last ones first
-  // (they see the most keys)
+  // ---- which sequence and tile: the tiles of all sequences counted off, all heads of one together, the last
+  // tiles first (they see the most keys; what starts last is short)
   if (warp == 0) {
-    int left = blockIdx.x, seq = -1, tile = 0, two = 1;
+    int left = blockIdx.x / c.heads, seq = -1, tile = 0, two = 1;
     for (int b0 = 0; b0 < c.B && seq < 0; b0 += 32) {
       const int b = b0 + lane;
       const int64_t r = b < c.B ? (int64_t)max(0, c.cu_new[b + 1] - c.cu_new[b]) * a.group : 0;
@@ -1004,10 +1004,10 @@ static int attend_plan(const AttendSizes &z, AttendPlan *p) {
   p->grid_tiles = 0;
   if (p->tiles) {
     const int64_t n = z.rows * group / tiles::ROWS + B;
-    if (n > INT32_MAX) return HIF4X_ERR_UNSUPPORTED;
+    if (n * H > INT32_MAX) return HIF4X_ERR_UNSUPPORTED;
     p->grid_tiles = (int)n;
-    // shares of the keys: as many as fill the SMs once, four steps or more to each
-    const int64_t busy = std::max<int64_t>(1, z.rows * group / tiles::ROWS) * H;
+    // shares of the keys: as many as fill the SMs once (sequences taken alike), four steps or more to each
+    const int64_t busy = B * std::max<int64_t>(1, (z.rows * group + B * tiles::ROWS - 1) / (B * tiles::ROWS)) * H;
     p->splits = (int)std::max<int64_t>(
         1, std::min<int64_t>({sms / busy, keys / (4 * tiles::KEYS), (int64_t(1) << 26) / (z.rows * z.q_heads * z.head_dim), MOST_SPLITS}));
   } else {
@@ -1025,7 +1025,7 @@ static int launch_tiles(AttendArgs a, int dev, const AttendPlan &p, cudaStream_t
   // the kernel compares unscaled scores, so its scale is positive: a negative one turns the queries' signs
   const int flip = a.scale < 0.0f;
   a.scale = std::max(std::fabs(a.scale), 1e-35f);
-  const dim3 grid((unsigned)p.grid_tiles, (unsigned)a.c.heads, (unsigned)p.splits);
+  const dim3 grid((unsigned)(p.grid_tiles * a.c.heads), (unsigned)p.splits);
   tiles::attend_tiles_kernel<DH><<<grid, tiles::THREADS, tiles::Cfg<DH>::SMEM, s>>>(a, flip);
   HIF4X_CHECK_LAUNCH();
   return HIF4X_OK;
