@@ -422,9 +422,8 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) attend_rows_kernel(const
 // scores, so the softmax goes by half steps of 64 keys: a tile's two halves
 // are two buffers, and while one is in the softmax the tensor core finishes
 // the other's second product and computes its next scores.  (With one buffer
-// of 128 keys a tile's softmax and products ran one after the other: 4820
-// cycles a step for the 2048 that each of the tensor core, the exponentials
-// and shared memory needs.)  The softmax reference moves as in
+// of 128 keys a tile's softmax and products ran one after the other: a
+// 2048-token chunk over 10240 keys took 447 us, now 380.)  The softmax reference moves as in
 // attend_rows_kernel, only past 2^8; then the row's O is rescaled in tensor
 // memory by the softmax warp, once the product before has finished.
 namespace tiles {
@@ -529,8 +528,8 @@ __device__ __forceinline__ void weights32(const uint32_t (&s)[32], u64 scale2, u
 // bits 0 .. n - 1 (none for n <= 0, all for n >= 64)
 __device__ __forceinline__ u64 below(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
 
-// Registers move from the warps that need few to the softmax: 256 x 144 +
-// 256 x 72 + 128 x 40 = 60416 of the launch's 640 x 96 = 61440.
+// Registers move from the warps that need few to the softmax: 256 x 152 +
+// 256 x 64 + 128 x 40 = 60416 of the launch's 640 x 96 = 61440.
 template <int N>
 __device__ __forceinline__ void regs_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -553,8 +552,8 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t *kfull = reinterpret_cast<uint64_t *>(smem + C::BARS), *kempty = kfull + 2, *vfull = kempty + 2;
   uint64_t *vempty = vfull + 2, *sfull = vempty + 2, *pfull = sfull + 4, *odone = pfull + 4;
-  uint64_t *drain = odone + 2, *turn = drain + 2;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(turn + 8);
+  uint64_t *drain = odone + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 2);
   int *found = reinterpret_cast<int *>(tmem_slot + 1);          // sequence, tile
   uint8_t *hidden = reinterpret_cast<uint8_t *>(found + 3);     // [4 steps][8 blocks of 16 keys]: 1 without a page
   const CacheArgs &c = a.c;
@@ -602,7 +601,6 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         mbar_init(&odone[i], 1);
         mbar_init(&drain[i], 1);
       }
-      for (int i = 0; i < 8; i++) mbar_init(&turn[i], 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
   }
@@ -658,7 +656,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
 
   if (warp >= 12) {
     // ---- decode
-    regs_down<72>();
+    regs_down<64>();
     const int w = warp - 12;
     const int *pages = c.pages + seq * c.ld_pages;
     const int last = p_hi;
@@ -710,7 +708,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
       auto qk = [&](int j) {
         const int st = (j >> 1) & 1;
         const uint64_t k = dk + st * (C::TILE >> 4) + (j & 1) * (64 * 128 >> 4);
-        ok = mbar_wait_sleep(&kfull[st], (j >> 2) & 1, c.status);
+        if (!(j & 1)) ok = mbar_wait_sleep(&kfull[st], (j >> 2) & 1, c.status);   // both halves at once
         if (!ok) return;
         tc_fence_after();
 #pragma unroll
@@ -727,8 +725,8 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
       for (int j = 0; j < 2 * n && ok; j++) {
         const int st = (j >> 1) & 1;
         const uint64_t v = dv + st * (C::TILE >> 4) + (j & 1) * (64 * 128 >> 4);
-        ok = mbar_wait_sleep(&vfull[st], (j >> 2) & 1, c.status) &&
-             mbar_wait_sleep(&pfull[2 * t + (j & 1)], (j >> 1) & 1, c.status);
+        if (!(j & 1)) ok = mbar_wait_sleep(&vfull[st], (j >> 2) & 1, c.status);
+        ok = ok && mbar_wait_sleep(&pfull[2 * t + (j & 1)], (j >> 1) & 1, c.status);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
@@ -747,7 +745,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
     __syncwarp();
   } else {
     // ---- softmax: this thread's row
-    regs_up<144>();
+    regs_up<152>();
     const int t = warp >> 2;
     const int r = t * 128 + (warp & 3) * 32 + lane;
     const int64_t rr = r0 + r;
@@ -820,20 +818,10 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         }
         const float base = ref == -INFINITY ? 0.0f : ref;
         const u64 scale2 = pk2(a.scale, a.scale), nref2 = pk2(-base, -base);
-        // the two warps of a scheduler, one of each tile, take turns at the exponentials: at the same time they
-        // would halve each other's rate and then leave both tiles to the tensor core at once
-        if (tiles_here == 2 && (t == 1 || j > 0)) {
-          ok = mbar_wait_sleep(&turn[warp ^ 4], (j - 1 + t) & 1, c.status);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tmem_loaded(s);   // the arithmetic stays behind the wait
-          tmem_loaded(s1);
-        }
         uint32_t w[32];
         weights32(s, scale2, nref2, sum2, w);
         weights32(s1, scale2, nref2, sum2, w + 16);
         tmem_st32(ts + 64 * h, w);   // over S columns that have been read
-        if (lane == 0) mbar_arrive(&turn[warp]);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
