@@ -423,9 +423,10 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) attend_rows_kernel(const
 // are two buffers, and while one is in the softmax the tensor core finishes
 // the other's second product and computes its next scores.  (With one buffer
 // of 128 keys a tile's softmax and products ran one after the other: a
-// 2048-token chunk over 10240 keys took 447 us, now 380.)  The softmax reference moves as in
-// attend_rows_kernel, only past 2^8; then the row's O is rescaled in tensor
-// memory by the softmax warp, once the product before has finished.
+// 2048-token chunk over 10240 keys took 447 us, now 380.)  The softmax
+// reference moves as in attend_rows_kernel, only past 2^8; then the row's O
+// is rescaled in tensor memory by the softmax warp, once the product before
+// has finished.
 namespace tiles {
 
 using namespace tc;
@@ -845,6 +846,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
 #pragma unroll 1
       for (int c0 = 0; c0 < DH; c0 += 32) {
         uint32_t o[32];
+        __syncwarp();   // lanes of rows that are not stored are ahead
         if (n > 0) {
           tmem_ld32(to + c0, o);
           tmem_wait_ld(o);
