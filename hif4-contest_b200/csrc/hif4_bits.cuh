@@ -65,6 +65,13 @@ __device__ __forceinline__ void hif4_scales(const Hif4Levels &l, uint32_t sf2, u
   s1 = mad32(l.l3 & (2u << (2 * J)), 0x00800080u >> (2 * J + 1), b);
 }
 
+// The same as one pair: quad 0's scale in the low half, quad 1's in the high one.
+template <int J>
+__device__ __forceinline__ uint32_t hif4_scale_pair(const Hif4Levels &l, uint32_t sf2) {
+  const uint32_t b = mad32(l.l2 & (1u << J), 0x00800080u >> J, sf2);
+  return mad32(l.l3 & (1u << (2 * J)), 0x80u >> (2 * J), mad32(l.l3 & (2u << (2 * J)), 0x00800000u >> (2 * J + 1), b));
+}
+
 // Word of sub-block i0 + J -> four bf16 pairs in element order (0,1) (2,3) (4,5) (6,7).
 template <int J>
 __device__ __forceinline__ void hif4_decode8(uint32_t w, const Hif4Levels &l, uint32_t sf2, uint32_t *o) {

@@ -73,12 +73,17 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// hif4_scales of sub-block j, an index that unrolling makes constant
+// hif4_scales and hif4_scale_pair of sub-block j, an index that unrolling makes constant
 __device__ __forceinline__ void scales_of(const Hif4Levels &l, uint32_t sf2, int j, uint32_t &s0, uint32_t &s1) {
   if (j == 0) hif4_scales<0>(l, sf2, s0, s1);
   else if (j == 1) hif4_scales<1>(l, sf2, s0, s1);
   else if (j == 2) hif4_scales<2>(l, sf2, s0, s1);
   else hif4_scales<3>(l, sf2, s0, s1);
+}
+
+__device__ __forceinline__ uint32_t scale_pair_of(const Hif4Levels &l, uint32_t sf2, int j) {
+  return j == 0 ? hif4_scale_pair<0>(l, sf2) : j == 1 ? hif4_scale_pair<1>(l, sf2)
+       : j == 2 ? hif4_scale_pair<2>(l, sf2) : hif4_scale_pair<3>(l, sf2);
 }
 
 // The 16-key tiles a run of positions [p_lo, p_hi] of one sequence can see:
@@ -240,6 +245,10 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) attend_rows_kernel(const
       cur.load_k(row_of(t, pg));
       cur.load_v(row_of(t, pg));
     }
+    // Two tiles a turn: the words loaded ahead need no moves between registers
+    // (64 sequences of up to 8192 keys: 169 us, one a turn 177; three and four
+    // a turn 195 and 250).
+#pragma unroll 2
     for (; t < t1; t += WARPS) {
       const int pg_next2 = page_of(t + 2 * WARPS);
       const int64_t row_next = pg_next >= 0 ? row_of(t + WARPS, pg_next) : 0;
@@ -256,10 +265,7 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) attend_rows_kernel(const
         const Hif4Levels l0(cur.km[0], i0), l1(cur.km[1], i0);
 #pragma unroll
         for (int w = 0; w < KW; w++) {
-          uint32_t a0, a1, b0, b1;
-          scales_of(l0, sf0, w, a0, a1);
-          scales_of(l1, sf1, w, b0, b1);
-          const uint32_t s0 = __byte_perm(a0, a1, 0x5410), s1 = __byte_perm(b0, b1, 0x5410);
+          const uint32_t s0 = scale_pair_of(l0, sf0, w), s1 = scale_pair_of(l1, sf1, w);
           const uint32_t z0 = bf16x2_mul(s0, kNeg136), z1 = bf16x2_mul(s1, kNeg136);
           const uint32_t x0 = hif4_offset(cur.k[0][w]), x1 = hif4_offset(cur.k[1][w]);
           uint32_t f[4][2];
@@ -948,7 +954,7 @@ __global__ void __launch_bounds__(128) attend_join_kernel(const AttendArgs a) {
 // lanes (sequence, key head): as many shares as the SMs hold CTAs at once (a
 // second wave would leave most of them idle; 65536 keys of one sequence: 50
 // us, 91 with three waves).  Many: twelve CTAs for every SM, so that sequences
-// of several lengths even out (64 sequences of up to 8192 keys: 180 us, 289
+// of several lengths even out (64 sequences of up to 8192 keys, one tile a turn: 180 us, 289
 // unshared).  No share under 512 keys (eight tiles for each warp; the join is
 // a launch of its own, 4 us), and no more than 2^26 partial sums (256 MB) in
 // all.
