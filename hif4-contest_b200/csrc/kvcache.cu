@@ -159,6 +159,14 @@ __device__ __forceinline__ void choose(const float (&a)[8], float amax, int lane
       lv = bits;
     }
   }
+  // A NaN compares with nothing.  With clamped scales the definition
+  // (csrc/codec.cu search_generic) keeps the smaller unit where its error is
+  // "<=", so a quad with a NaN takes the larger one; without, it takes the
+  // larger one where the smaller's error is ">", so there it does not.
+  if (!fast) {
+    if (!(a[0] + a[1] + a[2] + a[3] >= 0.0f)) lv |= 2u;
+    if (!(a[4] + a[5] + a[6] + a[7] >= 0.0f)) lv |= 4u;
+  }
 }
 
 __global__ void __launch_bounds__(128) append_kernel(const AppendArgs p) {
