@@ -49,6 +49,13 @@ struct AttendArgs {
   float2 *part_ml;
 };
 
+// Rows (token, query head of a key head) that the call's tensors have of a
+// sequence with n_new rows from cu0 on: the batch may be described beyond them.
+__device__ __forceinline__ int64_t rows_present(const AttendArgs &a, int cu0, int n_new) {
+  if (n_new <= 0 || cu0 < 0 || cu0 >= a.c.rows) return 0;
+  return min((int64_t)n_new, a.c.rows - cu0) * a.group;
+}
+
 constexpr int64_t MOST_SPLITS = 64;   // shares of a row's keys (attend_join_kernel: four warps, a lane for each of 16)
 constexpr float kLazy = 8.0f;    // log2 a row's scores may pass its reference by
 
@@ -170,12 +177,11 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) attend_rows_kernel(const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n8 = lane >> 2, q4 = lane & 3;
   const int s = blockIdx.x, kh = blockIdx.y, split = blockIdx.z;
   const int cu0 = c.cu_new[s], n_new = c.cu_new[s + 1] - cu0;
-  if (n_new <= 0) return;
+  const int64_t rows = rows_present(a, cu0, n_new);
+  if (rows == 0 || (int64_t)n_new * a.group > a.most_rows) return;
   const int64_t room = (int64_t)c.most << c.page_shift;
   const int old = c.kv_len[s] - n_new;   // position of the first new row
   const int *pages = c.pages + s * c.ld_pages;
-  if (cu0 < 0 || cu0 >= c.rows || (int64_t)n_new * a.group > a.most_rows) return;
-  const int64_t rows = min((int64_t)n_new, c.rows - cu0) * a.group;   // rows that the batch's tensors do not have: none
 
   for (int64_t r0 = 0; r0 < rows; r0 += ROWS) {
     const int64_t r1 = min(rows, r0 + ROWS);
@@ -573,8 +579,10 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
     int left = blockIdx.x / c.heads, seq = -1, tile = 0, two = 1;
     for (int b0 = 0; b0 < c.B && seq < 0; b0 += 32) {
       const int b = b0 + lane;
-      const int64_t r = b < c.B ? (int64_t)max(0, c.cu_new[b + 1] - c.cu_new[b]) * a.group : 0;
-      const int n = r > a.most_rows ? (int)((r + ROWS - 1) / ROWS) : 0;
+      const int at = b < c.B ? c.cu_new[b] : 0, count = b < c.B ? c.cu_new[b + 1] - at : 0;
+      // no more than the grid was sized for: the rows that are there
+      const int64_t r = (int64_t)count * a.group > a.most_rows ? rows_present(a, at, count) : 0;
+      const int n = (int)((r + ROWS - 1) / ROWS);
       int sum = n;
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) {
@@ -621,7 +629,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   const int cu0 = c.cu_new[seq], n_new = c.cu_new[seq + 1] - cu0, old = c.kv_len[seq] - n_new;
-  const int64_t rows = (int64_t)n_new * a.group, r0 = (int64_t)found[1] * ROWS;
+  const int64_t rows = rows_present(a, cu0, n_new), r0 = (int64_t)found[1] * ROWS;
   const int tiles_here = rows - r0 > 128 ? 2 : 1;
   const int64_t r1 = min(rows, r0 + ROWS);
   const int p_lo = old + (int)(r0 / a.group), p_top = old + (int)((r1 - 1) / a.group);

@@ -44,3 +44,39 @@ def test_append_of_values_that_are_none(dtype):
     linalg.check_device_status()
 
 
+# ------------------------------------------------------------------ rows that the tensors do not have
+def cut(b, rows):
+    """The batch of b's first `rows` rows: later rows and the keys only they see are gone."""
+    c, left = copy.copy(b), rows
+    c.new, c.lens = [], []
+    for n, full in zip(b.new, b.lens):
+        have = min(n, left)
+        left -= have
+        c.new.append(have)
+        c.lens.append(full - n + have)
+    return c
+
+
+@pytest.mark.parametrize("new,lens,qh,kvh,dh,rows", [
+    ([40, 60], [100, 200], 4, 2, 64, 70),               # the last sequence is cut
+    ([300, 300], [2000, 5000], 8, 2, 128, 200),         # and the one after it has no rows at all
+    ([300], [700], 4, 1, 64, 100),                      # most of a sequence is cut
+    ([2000, 60], [2000, 200], 8, 2, 128, 100),
+    ([300], [9000], 4, 1, 128, 100),                    # with the keys in shares
+    ([64, 64], [9000, 9000], 4, 1, 128, 70),
+    ([1, 64, 100, 2], [700, 64, 3000, 9], 8, 4, 64, 90),
+    ([20] * 8, list(range(40, 840, 100)), 8, 1, 64, 50),
+    ([1, 1, 1], [900, 33, 5000], 4, 2, 128, 2)])        # single tokens
+def test_rows_the_tensors_do_not_have(new, lens, qh, kvh, dh, rows):
+    """A batch description that goes on behind the rows of q: the rows that q has come out right, whatever
+    kernel takes them."""
+    b = Batch(new, lens, kvh, dh, 16, 41)
+    q = torch.randn(rows, qh, dh, generator=gen(rows), device="cuda").bfloat16()
+    c = cut(b, rows)
+    for most in (max(new), None, 1):
+        out = torch.full_like(q, float("nan"))
+        serve.paged_attention(q, b.cache, *b.args, max_new=most, out=out)
+        linalg.check_device_status()
+        check_attention(c, q, out)
+
+
