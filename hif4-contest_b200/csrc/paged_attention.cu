@@ -680,10 +680,17 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
     const Loader<DH> ld(c, kh, w, lane);
     Words<DH> cur, next;
     auto key_of = [&](int i) { return kt.key0(first + i, KEYS) + w * 16; };
-    auto look = [&](int i) { return i < n && key_of(i) <= last ? __ldg(pages + (key_of(i) >> c.page_shift)) : -1; };
-    auto check = [&](int i, int page) {   // an id of no page: -1, and reported where the keys exist
+    // whether a row of this CTA sees a key of the 16: steps of 128 begin before the window and end behind the sinks,
+    // and pages there may have been given back
+    const int before = a.window ? p_lo - a.window : INT32_MIN;
+    auto seen = [&](int i) {
+      const int k = key_of(i);
+      return i < n && k <= last && (k + 15 > before || k < a.sinks);
+    };
+    auto look = [&](int i) { return seen(i) ? __ldg(pages + (key_of(i) >> c.page_shift)) : -1; };
+    auto check = [&](int i, int page) {   // an id of no page: -1, and reported where a row would have seen the keys
       if (page >= 0 && page < c.num_pages) return page;
-      if (lane == 0 && i < n && key_of(i) <= last) atomicExch(c.status, HIF4X_BAD_PAGE);
+      if (lane == 0 && seen(i)) atomicExch(c.status, HIF4X_BAD_PAGE);
       return -1;
     };
     int now = look(0), nxt = look(1);   // of the step being decoded, of the one after it

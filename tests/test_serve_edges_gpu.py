@@ -80,3 +80,31 @@ def test_rows_the_tensors_do_not_have(new, lens, qh, kvh, dh, rows):
         check_attention(c, q, out)
 
 
+# ------------------------------------------------------------------ pages that no row sees
+@pytest.mark.parametrize("page", [16, 32, 128])
+@pytest.mark.parametrize("new,lens,qh,kvh,dh", [([1, 2], [3000, 700], 4, 2, 128),            # few rows
+                                                ([60, 200], [3000, 1531], 4, 2, 128),        # tiles
+                                                ([300, 1], [2047, 1999], 8, 8, 64),          # both
+                                                ([70], [5000], 4, 1, 128)])                  # keys in shares
+@pytest.mark.parametrize("window,sinks", [(100, 0), (100, 4), (1024, 20), (1, 130), (333, 1)])
+def test_pages_that_no_row_sees_may_be_none(new, lens, qh, kvh, dh, page, window, sinks):
+    """Table entries of pages that hold no visible key (those outside the window and the sinks, given back) may name
+    no page: the result is right and nothing is reported."""
+    b = Batch(new, lens, kvh, dh, page, 42)
+    q = torch.randn(b.rows, qh, dh, generator=gen(window), device="cuda").bfloat16()
+    table = b.pages.clone()
+    freed = 0
+    for i, (n, full) in enumerate(zip(new, lens)):
+        p, t = np.arange(full - n, full)[:, None], np.arange(full)[None]
+        seen = ((t <= p) & ((t > p - window) | (t < sinks))).any(0)
+        for j in range(-(-full // page)):
+            if not seen[j * page:(j + 1) * page].any():
+                table[i, j] = -1
+                freed += 1
+    assert freed > 0
+    for most in (max(new), None):
+        out = serve.paged_attention(q, b.cache, b.cu, b.len, table, window=window, sinks=sinks, max_new=most)
+        linalg.check_device_status()
+        check_attention(b, q, out, window, sinks)
+
+
