@@ -73,11 +73,14 @@ static_assert(Tile<256>::TMEM_COLS <= 512, "tensor memory columns");
 // blocks on side streams) from 106.3 to 104 ms; 8, 24 and 36 did less well
 constexpr int kTcFreeSms = 16;
 
-__device__ int g_status;   // sticky device status: 0 or HIF4X_TIMEOUT
+// Sticky device status: [0] 0 or HIF4X_TIMEOUT, from the bounded waits of every
+// kernel; [1] 0 or HIF4X_BAD_PAGE, from those that follow a page table.  Two
+// words, as the second is one caller's mistake and voids no other's results.
+__device__ int g_status[2];
 
 // bounded wait: false (and the device status set) if the phase never completes
 __device__ __forceinline__ bool mbar_wait_limit(uint64_t *bar, uint32_t parity, long long limit) {
-  return mbar_wait_limit(bar, parity, limit, &g_status);
+  return mbar_wait_limit(bar, parity, limit, g_status);
 }
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
   return mbar_wait_limit(bar, parity, SPIN_LIMIT);
@@ -753,9 +756,9 @@ int gemm_split(const float *As, int a_products, const float *Bs, int b_products,
   return cudaGetLastError() == cudaSuccess ? HIF4X_OK : HIF4X_ERR_LAUNCH;
 }
 
-// Device address of the sticky status word on device `dev` (the current one),
+// Device address of the two status words on device `dev` (the current one),
 // looked up once; null on failure, which the next call tries again.
-int *status_word(int dev) {
+int *status_words(int dev) {
   static std::mutex lock;
   static int *word[kMaxDevices];
   if (dev < 0 || dev >= kMaxDevices) return nullptr;
@@ -833,16 +836,24 @@ extern "C" int hif4x_wait_selftest(long long spins, int *done_dev, void *stream)
   return cudaStreamSynchronize((cudaStream_t)stream) == cudaSuccess ? HIF4X_OK : HIF4X_ERR_LAUNCH;
 }
 
-// Synchronises the stream and reports (then clears) the sticky device status
-// set by bounded waits that expired: HIF4X_OK or HIF4X_TIMEOUT.  The word is
-// one per device, not per stream: a read from any stream clears it for all.
-extern "C" int hif4x_device_status(void *stream) {
+// Synchronises the stream, reads the first `words` status words and reports
+// (then clears) the first that is set.  The words are one pair per device, not
+// per stream: a read from any stream clears for all.
+static int read_status(int words, void *stream) {
   if (cudaStreamSynchronize((cudaStream_t)stream) != cudaSuccess) return HIF4X_ERR_LAUNCH;
-  int st = 0;
-  if (cudaMemcpyFromSymbol(&st, tc::g_status, sizeof(int)) != cudaSuccess) return HIF4X_ERR_LAUNCH;
-  if (st != 0) {
-    const int zero = 0;
-    cudaMemcpyToSymbol(tc::g_status, &zero, sizeof(int));
-  }
-  return st;
+  int st[2] = {0, 0};
+  if (cudaMemcpyFromSymbol(st, tc::g_status, words * sizeof(int)) != cudaSuccess) return HIF4X_ERR_LAUNCH;
+  for (int w = 0; w < words; w++)
+    if (st[w] != 0) {
+      const int zero = 0;
+      cudaMemcpyToSymbol(tc::g_status, &zero, sizeof(int), w * sizeof(int));
+      return st[w];
+    }
+  return HIF4X_OK;
 }
+
+// HIF4X_OK, HIF4X_TIMEOUT, or HIF4X_BAD_PAGE where no wait has expired
+extern "C" int hif4x_device_status(void *stream) { return read_status(2, stream); }
+
+// HIF4X_OK or HIF4X_TIMEOUT: what a conversion asks, which no page table concerns
+extern "C" int hif4x_wait_status(void *stream) { return read_status(1, stream); }

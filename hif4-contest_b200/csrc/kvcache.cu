@@ -32,7 +32,7 @@ __device__ __forceinline__ int64_t cache_row(const CacheArgs &a, int64_t token, 
   const int64_t at = pos >> a.page_shift;
   const int64_t page = at < a.most ? (int64_t)a.pages[s * a.ld_pages + at] : -1;
   if (page < 0 || page >= a.num_pages) {
-    atomicExch(a.status, HIF4X_BAD_PAGE);
+    atomicExch(a.status + 1, HIF4X_BAD_PAGE);
     return -1;
   }
   return (page * a.heads + head) * a.page_size + (pos & (a.page_size - 1));
@@ -314,7 +314,7 @@ int cache_args(const hif4x_kv_cache *kv, const hif4x_kv_batch *b, int64_t rows, 
   a->most = b->max_pages;
   a->ld_pages = b->ld_pages;
   a->rows = rows;
-  a->status = tc::status_word(dev);
+  a->status = tc::status_words(dev);
   return a->status ? HIF4X_OK : HIF4X_ERR_LAUNCH;
 }
 

@@ -12,7 +12,7 @@ struct CacheArgs {
   const int *cu_new, *kv_len, *pages;
   int B, most;           // sequences; entries of a row of `pages` that count
   int64_t ld_pages, rows;
-  int *status;
+  int *status;           // [0] of the bounded waits, [1] of the page tables
 };
 
 // csrc/kvcache.cu: checks a cache and batch description and fills the arguments

@@ -353,7 +353,7 @@ extern "C" int hif4x_linear_packed(const void *x, int64_t ldx, const uint32_t *m
   if (sms <= 0 || dev >= kMaxDevices) return HIF4X_ERR_LAUNCH;
   static SharedOptIn opt_in;
   Args a{};
-  a.status = status_word(dev);
+  a.status = status_words(dev);
   if (!opt_in(linear_kernel, smem_bytes(256), dev) || !a.status) return HIF4X_ERR_LAUNCH;
 
   const int64_t tiles_n = (N + BM - 1) / BM;

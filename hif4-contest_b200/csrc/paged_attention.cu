@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) attend_rows_kernel(const
     const int p_top = old + (int)((r1 - 1) / a.group);
     int p_hi = p_top;
     if (p_hi >= room) {   // the table has no page for its last keys
-      if (threadIdx.x == 0) atomicExch(c.status, HIF4X_BAD_PAGE);
+      if (threadIdx.x == 0) atomicExch(c.status + 1, HIF4X_BAD_PAGE);
       p_hi = (int)(room - 1);
     }
     // this thread's Q fragments: row r0 + 8 nt + n8, dims q4 dh/4 .. in pairs (j, j + 4)
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) attend_rows_kernel(const
       if (i >= t1) return -1;
       const int pg = __ldg(pages + (tiles.key0(i, 16) >> c.page_shift));
       if (pg >= 0 && pg < c.num_pages) return pg;
-      if (lane == 0) atomicExch(c.status, HIF4X_BAD_PAGE);
+      if (lane == 0) atomicExch(c.status + 1, HIF4X_BAD_PAGE);
       return -1;
     };
     auto row_of = [&](int i, int pg) -> int64_t {
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
   const int64_t room = (int64_t)c.most << c.page_shift;
   int p_hi = p_top;
   if (p_hi >= room) {
-    if (threadIdx.x == 0) atomicExch(c.status, HIF4X_BAD_PAGE);
+    if (threadIdx.x == 0) atomicExch(c.status + 1, HIF4X_BAD_PAGE);
     p_hi = (int)(room - 1);
   }
   const KeyTiles kt(min(max(p_lo, 0), p_hi), p_hi, a.window, a.sinks, KEYS);
@@ -690,7 +690,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
     auto look = [&](int i) { return seen(i) ? __ldg(pages + (key_of(i) >> c.page_shift)) : -1; };
     auto check = [&](int i, int page) {   // an id of no page: -1, and reported where a row would have seen the keys
       if (page >= 0 && page < c.num_pages) return page;
-      if (lane == 0 && seen(i)) atomicExch(c.status, HIF4X_BAD_PAGE);
+      if (lane == 0 && seen(i)) atomicExch(c.status + 1, HIF4X_BAD_PAGE);
       return -1;
     };
     int now = look(0), nxt = look(1);   // of the step being decoded, of the one after it

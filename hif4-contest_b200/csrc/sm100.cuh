@@ -16,9 +16,10 @@ namespace tc {
 constexpr long long SPIN_LIMIT = 1ll << 22;   // polls of a device-side wait before it gives up
 constexpr int kMaxDevices = 64;
 
-// csrc/gemm_tc.cu: SM count of a device (0 on failure), its sticky status word (null on failure)
+// csrc/gemm_tc.cu: SM count of a device (0 on failure), its sticky status words (null on failure): [0] of the
+// bounded waits, [1] of the page tables
 int device_sms(int dev);
-int *status_word(int dev);
+int *status_words(int dev);
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

@@ -19,10 +19,19 @@ def _s(t: torch.Tensor):
 
 def check_device_status(dev=None) -> None:
     """Raise if, since the last check, a bounded device-side wait expired or a
-    page table named no page of a key/value cache."""
+    page table named no page of a key/value cache (where both did, the next
+    check tells of the page)."""
     st = L.lib().hif4x_device_status(L.stream(dev))
     if st != L.OK:
         raise L.Hif4xError("hif4x_device_status", st if st < 0 or st == L.BAD_PAGE else -st)
+
+
+def check_waits(dev=None) -> None:
+    """Raise if a bounded device-side wait expired since the last check; what a
+    page table did stays for check_device_status."""
+    st = L.lib().hif4x_wait_status(L.stream(dev))
+    if st != L.OK:
+        raise L.Hif4xError("hif4x_wait_status", st if st < 0 else -st)
 
 
 def gemm(A: torch.Tensor, B: torch.Tensor, *, ta: bool = False, tb: bool = False, alpha: float = 1.0,

@@ -528,7 +528,7 @@ def calibrate_weight(weight_quant: torch.Tensor, weight_scale: torch.Tensor, cal
         info["phases_ms"] = ph.result()
         info.update(alpha=best_alpha, mode=mode, gptq_w=gptq_w, gptq_act=gptq_act, e3=refined, tmax=tmax,
                     w_final=w_final, q_used=q_used, s=s)
-    la.check_device_status(dev)
+    la.check_waits(dev)
     out = (lambda t: t) if return_device else hostio.to_host
     activation_state = {
         "s": out(s),
@@ -718,5 +718,5 @@ def dynamic_activation(activation_quant: torch.Tensor, activation_scale: torch.T
                 result = None
     if result is None:
         result = codec.values_to_params(values, p) if values is not None else p
-    la.check_device_status(dev)
+    la.check_waits(dev)
     return result if return_device else result.reference()

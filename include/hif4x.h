@@ -206,10 +206,15 @@ int hif4x_gemm_tc(int ta, int tb, int64_t M, int64_t N, int64_t K, float alpha, 
  * HIF4X_TIMEOUT if a bounded device-side wait expired since the last call,
  * HIF4X_BAD_PAGE if a kernel of the key/value cache met a position whose page
  * table entry names no page (the row is not written, the keys count as
- * hidden); the later of the two where both happened.
- * One status word per device (not per stream): a read clears it for every
- * stream of that device. */
+ * hidden).  Where both happened the first call returns (and clears)
+ * HIF4X_TIMEOUT, the next one HIF4X_BAD_PAGE.
+ * One status per device (not per stream): a read clears it for every stream
+ * of that device. */
 int hif4x_device_status(void *stream);
+
+/* The same for the bounded waits alone: HIF4X_TIMEOUT or 0.  What a page table
+ * did stays for hif4x_device_status. */
+int hif4x_wait_status(void *stream);
 
 /* Failure-path check of the bounded device-side wait (no counterpart in the
  * reference, which has no device code): one thread waits `spins` polls

@@ -108,3 +108,45 @@ def test_pages_that_no_row_sees_may_be_none(new, lens, qh, kvh, dh, page, window
         check_attention(b, q, out, window, sinks)
 
 
+# ------------------------------------------------------------------ the device status
+def bad_page():
+    """One append whose page is none."""
+    cache = serve.PagedKV.empty(2, 16, 1, 64, "cuda")
+    x = torch.ones(1, 1, 64, device="cuda").bfloat16()
+    cu, one, table = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([0, 1], [1], [[5]]))
+    serve.kv_append(cache, x, x, cu, one, table)
+
+
+def test_a_bad_page_is_not_the_conversions_affair():
+    """A conversion on the same device neither fails for a serving call's bad page nor takes its report."""
+    from hif4x import linear, synth
+    pair = synth.nvfp4_pair(synth.codec_c1(3, 8, 128))
+    linalg.check_device_status()
+    bad_page()
+    linear.dynamic_activation(*pair, None)
+    with pytest.raises(L.Hif4xError, match="page"):
+        linalg.check_device_status()
+    linalg.check_device_status()
+
+
+@pytest.mark.parametrize("first", ["wait", "page"])
+def test_a_bad_page_does_not_hide_an_expired_wait(first):
+    """Both are reported, the expired wait (whose results are void) first, whichever came first."""
+    status = lambda: L.lib().hif4x_device_status(L.stream())  # noqa: E731
+    done = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert status() == L.OK
+    wait = lambda: L.lib().hif4x_wait_selftest(1000, L.ptr(done), L.stream())  # noqa: E731
+    for event in (wait, bad_page) if first == "wait" else (bad_page, wait):
+        event()
+    assert [status() for _ in range(3)] == [L.TIMEOUT, L.BAD_PAGE, L.OK]
+
+
+def test_a_conversion_still_learns_of_an_expired_wait():
+    from hif4x import linear, synth
+    done = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert L.lib().hif4x_wait_selftest(1000, L.ptr(done), L.stream()) == L.OK
+    with pytest.raises(L.Hif4xError):
+        linear.dynamic_activation(*synth.nvfp4_pair(synth.codec_c1(3, 8, 128)), None)
+    linalg.check_device_status()
+
+
