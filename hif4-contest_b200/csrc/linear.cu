@@ -76,14 +76,19 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// 1 / (1 + exp(-z)) without a sum that cancels or an exponential out of range:
+// a few steps of its own size on both sides of zero.
+__device__ __forceinline__ float sigmoid(float z) {
+  const float e = expf(-fabsf(z));
+  return (z < 0.0f ? e : 1.0f) / (1.0f + e);
+}
+
 __device__ __forceinline__ float activate(float v, int act) {
   switch (act) {
     case HIF4X_ACT_RELU: return v > 0.0f ? v : (v != v ? v : 0.0f);
     case HIF4X_ACT_GELU: return v * normcdff(v);
-    case HIF4X_ACT_GELU_TANH: {
-      const float z = 0.7978845608028654f * (v + 0.044715f * v * v * v);
-      return 0.5f * v * (1.0f + tanhf(z));
-    }
+    case HIF4X_ACT_GELU_TANH:   // (1 + tanh(z)) / 2 = 1 / (1 + exp(-2z))
+      return v * sigmoid(2.0f * 0.7978845608028654f * (v + 0.044715f * v * v * v));
     case HIF4X_ACT_SILU: return v / (1.0f + expf(-v));
     default: return v;
   }

@@ -150,3 +150,23 @@ def test_a_conversion_still_learns_of_an_expired_wait():
     linalg.check_device_status()
 
 
+# ------------------------------------------------------------------ far arguments of the activations
+def activation_of(v, act):
+    """act(v) by serve.linear: a weight of zeros and the bias v, so nothing is rounded before the activation."""
+    n = v.numel()
+    x = torch.ones(1, 64, device="cuda").bfloat16()
+    meta, codes = torch.zeros(n, 1, dtype=torch.int32, device="cuda"), torch.zeros(n, 32, dtype=torch.uint8, device="cuda")
+    return serve.linear(x, meta, codes, bias=v, activation=act)[0].double()
+
+
+def test_gelu_tanh_of_negative_arguments():
+    """One rounding to bf16 is all that a value far left of zero loses.  2z carries up to eight fp32 half steps, which the exponential
+    turns into 2|z| times as many of its own; exp, sum and quotient add a few."""
+    v = torch.cat((torch.linspace(-9, 0, 4001), torch.linspace(0, 12, 501))).cuda()
+    z = math.sqrt(2 / math.pi) * (v.double() + 0.044715 * v.double() ** 3)
+    want = v.double() * torch.sigmoid(2 * z)
+    tol = want.abs() * (BF16 * 1.01 + (8 * 2 * z.abs() + 16) * 2.0 ** -24)
+    off = (activation_of(v, "gelu_tanh") - want).abs()
+    assert (off <= tol).all(), f"off by {(off / tol.clamp_min(1e-300)).max().item():.2f} of the tolerance"
+
+
