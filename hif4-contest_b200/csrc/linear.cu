@@ -89,7 +89,7 @@ __device__ __forceinline__ float activate(float v, int act) {
     case HIF4X_ACT_GELU: return v * normcdff(v);
     case HIF4X_ACT_GELU_TANH:   // (1 + tanh(z)) / 2 = 1 / (1 + exp(-2z))
       return v * sigmoid(2.0f * 0.7978845608028654f * (v + 0.044715f * v * v * v));
-    case HIF4X_ACT_SILU: return v / (1.0f + expf(-v));
+    case HIF4X_ACT_SILU: return v * sigmoid(v);
     default: return v;
   }
 }

@@ -170,3 +170,14 @@ def test_gelu_tanh_of_negative_arguments():
     assert (off <= tol).all(), f"off by {(off / tol.clamp_min(1e-300)).max().item():.2f} of the tolerance"
 
 
+def test_silu_of_far_negative_arguments():
+    """Down to where bf16 has no value left (half its last step is 2^-134), the result is the formula's: exp(-v) passes
+    fp32's range at v = -88.7, the result bf16's smallest normal value only behind it."""
+    v = torch.cat((torch.linspace(-110, -80, 6001), torch.linspace(-80, 110, 1901))).cuda()
+    want = v.double() * torch.sigmoid(v.double())
+    # exp within two steps of fp32 (2^-149 each where it has no more bits), product and quotient half a step each
+    tol = want.abs() * (BF16 * 1.01 + 16 * 2.0 ** -24) + 1.01 * 2.0 ** -134 + 4 * v.double().abs() * 2.0 ** -149
+    off = (activation_of(v, "silu") - want).abs()
+    assert (off <= tol).all(), f"off by {(off / tol).max().item():.2f} of the tolerance"
+
+
