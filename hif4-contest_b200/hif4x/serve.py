@@ -64,13 +64,27 @@ def _row_stride(t: torch.Tensor, name: str, aligned: bool) -> int:
     return ld
 
 
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses from a tensor's first element to behind its last."""
+    at = t.data_ptr()
+    if t.is_contiguous():
+        return at, at + t.nbytes
+    return at, at + (sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the spans of two tensors' elements meet."""
-    def span(t):
-        n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1
-        return t.data_ptr(), t.data_ptr() + n * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
+    (a0, a1), (b0, b1) = _span(a), _span(b)
     return a0 < b1 and b0 < a1
+
+
+def _apart(out: torch.Tensor, name: str, *inputs) -> None:
+    """`out` lies over none of the inputs, (tensor or span, name) each."""
+    o0, o1 = _span(out)
+    for t, what in inputs:
+        a0, a1 = t if isinstance(t, tuple) else _span(t)
+        if o0 < a1 and a0 < o1:
+            raise ValueError(f"{name} overlaps {what}")
 
 
 def linear(x: torch.Tensor, meta: torch.Tensor, codes: torch.Tensor, bias: torch.Tensor | None = None,
@@ -81,7 +95,7 @@ def linear(x: torch.Tensor, meta: torch.Tensor, codes: torch.Tensor, bias: torch
     x: (T, C) bf16, unit inner stride, rows a multiple of 8 elements apart, 16-byte aligned.  meta int32
     (N, C/64) and codes uint8 (N, C/2): contiguous.  bias: (N,) fp32 or bf16.  activation: none, relu, gelu
     (by erf), gelu_tanh or silu.  residual: (T, N) bf16, unit inner stride; out: the same, and it may be the
-    residual itself, not x.  Sums are fp32 on the tensor cores, rounded once at the end."""
+    residual itself, but lie over no other input.  Sums are fp32 on the tensor cores, rounded once at the end."""
     _cuda(x, "x", (torch.bfloat16,), 2)
     dev = x.device
     _cuda(codes, "codes", (torch.uint8,), 2, dev)
@@ -120,8 +134,8 @@ def linear(x: torch.Tensor, meta: torch.Tensor, codes: torch.Tensor, bias: torch
         if out.shape != (T, N):
             raise ValueError(f"out is {tuple(out.shape)}: ({T}, {N}) wanted")
         ldy = _row_stride(out, "out", False)
-        if T and _overlap(out, x):
-            raise ValueError("out overlaps x")
+        if T:
+            _apart(out, "out", (x, "x"), (meta, "meta"), (codes, "codes"), *([(bias, "bias")] if bias is not None else []))
         if T and residual is not None and _overlap(out, residual) and not (
                 out.data_ptr() == residual.data_ptr() and ldy == ldr):
             raise ValueError("out overlaps residual without being it")
@@ -163,6 +177,7 @@ class PagedKV:
             raise ValueError("the cache has no pages or no heads")
         self.k_codes, self.k_meta, self.v_codes, self.v_meta = k_codes, k_meta, v_codes, v_meta
         self.num_pages, self.kv_heads, self.page_size, self.head_dim, self.device = n, h, p, 2 * half, dev
+        self._spans = [(_span(t), "the cache") for t in (k_codes, k_meta, v_codes, v_meta)]
         self._desc = L.KVCacheDesc(*at, n, p, h, 2 * half)
         self._ref = ctypes.byref(self._desc)
 
@@ -175,6 +190,10 @@ class PagedKV:
         make = lambda last, dt: torch.zeros(*shape, last, dtype=dt, device=device)  # noqa: E731
         return PagedKV(make(head_dim // 2, torch.uint8), make(head_dim // 64, torch.int32),
                        make(head_dim // 2, torch.uint8), make(head_dim // 64, torch.int32))
+
+    def _reads(self, cu_new: torch.Tensor, kv_len: torch.Tensor, pages: torch.Tensor):
+        """What a call over the cache reads besides its rows, for _apart."""
+        return *self._spans, (cu_new, "cu_new"), (kv_len, "kv_len"), (pages, "pages")
 
     def _batch(self, cu_new: torch.Tensor, kv_len: torch.Tensor, pages: torch.Tensor) -> L.KVBatchDesc:
         dev = self.device
@@ -235,8 +254,8 @@ def kv_read(cache: PagedKV, cu_new: torch.Tensor, kv_len: torch.Tensor, pages: t
             dtype: torch.dtype = torch.bfloat16, out: tuple[torch.Tensor, torch.Tensor] | None = None):
     """(k, v): the values of the batch's rows as the cache holds them, (rows, kv_heads, head_dim) of `dtype`
     (bf16 or fp32, both exact): the rows that kv_append writes for the same arguments, or any run of last
-    tokens that cu_new names.  out: tensors to write instead; rows that have no place are left as they were
-    (undefined without out)."""
+    tokens that cu_new names.  out: tensors to write instead, apart from all that is read; rows that have no place
+    are left as they were (undefined without out)."""
     batch = cache._batch(cu_new, kv_len, pages)
     if rows < 0:
         raise ValueError(f"rows {rows}")
@@ -249,8 +268,11 @@ def kv_read(cache: PagedKV, cu_new: torch.Tensor, kv_len: torch.Tensor, pages: t
         _heads(v, "out[1]", (k.dtype,), cache, cache.kv_heads)
         if k.shape[0] != rows or v.shape[0] != rows or not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError(f"out must be two contiguous tensors of {rows} rows")
-        if rows and (k.data_ptr() % 16 or v.data_ptr() % 16 or _overlap(k, v)):
-            raise ValueError("out must be two 16-byte aligned tensors apart")
+        if rows:
+            if k.data_ptr() % 16 or v.data_ptr() % 16 or _overlap(k, v):
+                raise ValueError("out must be two 16-byte aligned tensors apart")
+            for t, name in ((k, "out[0]"), (v, "out[1]")):
+                _apart(t, name, *cache._reads(cu_new, kv_len, pages))
     if rows:
         _call(cache.device, "hif4x_kv_read", cache._ref, ctypes.byref(batch), rows, k.data_ptr(),
               v.data_ptr(), L.dtype_code(k.dtype))
@@ -276,7 +298,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, cu_new: torch.Tensor, kv_le
     reads key head h // (q_heads / kv_heads).  A row that sees nothing (a negative position) gives zeros.
     scale: head_dim ** -0.5 by default.  max_new: the most new rows of a sequence, if the program knows it
     (rows otherwise): it chooses how the work is laid out; the result holds for any.  out: a tensor to write
-    instead, not q; rows of no sequence are left as they were (undefined without out)."""
+    instead, apart from all that is read; rows of no sequence are left as they were (undefined without out)."""
     _heads(q, "q", (torch.bfloat16,), cache)
     rows, heads, dh = q.shape
     if heads == 0 or heads % cache.kv_heads:
@@ -297,8 +319,10 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, cu_new: torch.Tensor, kv_le
         orow, ohead = _strides(out, "out")
         by_row = ohead >= dh and orow >= (heads - 1) * ohead + dh
         by_head = orow >= dh and ohead >= (rows - 1) * orow + dh
-        if rows and (_overlap(out, q) or not (by_row or by_head)):
-            raise ValueError("out overlaps q or itself")
+        if rows and not (by_row or by_head):
+            raise ValueError("out overlaps itself")
+        if rows:
+            _apart(out, "out", (q, "q"), *cache._reads(cu_new, kv_len, pages))
     if rows == 0:
         return out
     most = min(rows, max_new) if max_new is not None else rows

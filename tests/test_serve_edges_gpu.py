@@ -181,3 +181,32 @@ def test_silu_of_far_negative_arguments():
     assert (off <= tol).all(), f"off by {(off / tol).max().item():.2f} of the tolerance"
 
 
+# ------------------------------------------------------------------ tensors that overlap, and what is refused
+def test_out_overlaps_no_input():
+    """`out` may lie over no tensor that the call reads (in linear the residual itself excepted)."""
+    T, N, C = 4, 64, 128
+    meta, codes = packed(50, N, C)
+    x = torch.zeros(T, C, dtype=torch.bfloat16, device="cuda")
+    flat = torch.zeros(4096, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="overlaps bias"):
+        serve.linear(x, meta, codes, bias=flat[:N], out=flat[:T * N].view(T, N))
+    with pytest.raises(ValueError, match="overlaps codes"):
+        serve.linear(x, meta, flat.view(torch.uint8)[:N * C // 2].view(N, C // 2), out=flat[:T * N].view(T, N))
+    with pytest.raises(ValueError, match="overlaps meta"):
+        serve.linear(x, flat.view(torch.int32)[:N * C // 64].view(N, C // 64), codes, out=flat[:T * N].view(T, N))
+    b = Batch([2], [20], 2, 64, 16, 51)
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="cuda")
+    c = b.cache
+    for t in (c.k_codes, c.k_meta, c.v_codes, c.v_meta):
+        over = t.view(-1).view(torch.bfloat16)
+        if over.numel() < 512:
+            continue
+        with pytest.raises(ValueError, match="overlaps the cache"):
+            serve.paged_attention(q, c, *b.args, out=over[:512].view(2, 4, 64))
+        with pytest.raises(ValueError, match="overlaps the cache"):
+            serve.kv_read(c, *b.args, rows=2, out=(over[:256].view(2, 2, 64), torch.zeros(2, 2, 64, device="cuda").bfloat16()))
+    table = torch.zeros(1, 256, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="overlaps pages"):
+        serve.paged_attention(q, c, b.cu, b.len, table, out=table.view(torch.bfloat16).view(2, 4, 64))
+
+
