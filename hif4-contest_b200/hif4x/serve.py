@@ -78,12 +78,28 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def _runs(t: torch.Tensor) -> tuple[int, int]:
+    """(pitch, width) in bytes: the elements as runs of `width` that begin `pitch` apart, a run for each index of
+    the dimension with the largest stride."""
+    dims = sorted((st, s) for s, st in zip(t.shape, t.stride()) if s > 1)
+    size = t.element_size()
+    if not dims:
+        return 0, size
+    return dims[-1][0] * size, (sum((s - 1) * st for st, s in dims[:-1]) + 1) * size
+
+
+def _beside(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors whose spans meet are ranges of columns of one buffer that do not."""
+    (pa, wa), (pb, wb) = _runs(a), _runs(b)
+    if pa != pb or pa == 0:
+        return False
+    return wa <= (b.data_ptr() - a.data_ptr()) % pa <= pa - wb
+
+
 def _apart(out: torch.Tensor, name: str, *inputs) -> None:
-    """`out` lies over none of the inputs, (tensor or span, name) each."""
-    o0, o1 = _span(out)
+    """`out` lies over none of the inputs, (tensor, name) each."""
     for t, what in inputs:
-        a0, a1 = t if isinstance(t, tuple) else _span(t)
-        if o0 < a1 and a0 < o1:
+        if _overlap(out, t) and not _beside(out, t):
             raise ValueError(f"{name} overlaps {what}")
 
 
@@ -136,7 +152,7 @@ def linear(x: torch.Tensor, meta: torch.Tensor, codes: torch.Tensor, bias: torch
         ldy = _row_stride(out, "out", False)
         if T:
             _apart(out, "out", (x, "x"), (meta, "meta"), (codes, "codes"), *([(bias, "bias")] if bias is not None else []))
-        if T and residual is not None and _overlap(out, residual) and not (
+        if T and residual is not None and _overlap(out, residual) and not _beside(out, residual) and not (
                 out.data_ptr() == residual.data_ptr() and ldy == ldr):
             raise ValueError("out overlaps residual without being it")
     if T == 0:
@@ -177,7 +193,6 @@ class PagedKV:
             raise ValueError("the cache has no pages or no heads")
         self.k_codes, self.k_meta, self.v_codes, self.v_meta = k_codes, k_meta, v_codes, v_meta
         self.num_pages, self.kv_heads, self.page_size, self.head_dim, self.device = n, h, p, 2 * half, dev
-        self._spans = [(_span(t), "the cache") for t in (k_codes, k_meta, v_codes, v_meta)]
         self._desc = L.KVCacheDesc(*at, n, p, h, 2 * half)
         self._ref = ctypes.byref(self._desc)
 
@@ -193,7 +208,8 @@ class PagedKV:
 
     def _reads(self, cu_new: torch.Tensor, kv_len: torch.Tensor, pages: torch.Tensor):
         """What a call over the cache reads besides its rows, for _apart."""
-        return *self._spans, (cu_new, "cu_new"), (kv_len, "kv_len"), (pages, "pages")
+        cache = ((t, "the cache") for t in (self.k_codes, self.k_meta, self.v_codes, self.v_meta))
+        return *cache, (cu_new, "cu_new"), (kv_len, "kv_len"), (pages, "pages")
 
     def _batch(self, cu_new: torch.Tensor, kv_len: torch.Tensor, pages: torch.Tensor) -> L.KVBatchDesc:
         dev = self.device

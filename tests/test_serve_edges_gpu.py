@@ -210,3 +210,26 @@ def test_out_overlaps_no_input():
         serve.paged_attention(q, c, b.cu, b.len, table, out=table.view(torch.bfloat16).view(2, 4, 64))
 
 
+@pytest.mark.parametrize("T", [1, 5, 300])
+def test_out_beside_an_input_in_one_buffer(T):
+    """Two column ranges of one buffer never meet: x and out, residual and out, q and out may lie so."""
+    N, C = 96, 128
+    meta, codes = packed(52, N, C)
+    wide = torch.randn(T, C + 2 * N, generator=gen(T), device="cuda").bfloat16()
+    x, res, out = wide[:, :C], wide[:, C:C + N], wide[:, C + N:]
+    keep = wide.clone()
+    serve.linear(x, meta, codes, residual=res, out=out)
+    check_linear(x, meta, codes, out, res=res)
+    assert torch.equal(wide[:, :C + N], keep[:, :C + N])
+    b = Batch([T], [T + 40], 2, 64, 16, 53)
+    both = torch.randn(T, 2, 4, 64, generator=gen(T + 1), device="cuda").bfloat16()
+    q = both[:, 0].clone()
+    serve.paged_attention(both[:, 0], b.cache, *b.args, out=both[:, 1])
+    check_attention(b, q, both[:, 1])
+    assert torch.equal(both[:, 0], q)
+    # and ranges that do meet are refused
+    if T > 1:
+        with pytest.raises(ValueError, match="overlaps x"):
+            serve.linear(x, meta, codes, out=wide[:, C - 8:C - 8 + N])
+
+
