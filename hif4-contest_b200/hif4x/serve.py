@@ -166,7 +166,7 @@ def linear(x: torch.Tensor, meta: torch.Tensor, codes: torch.Tensor, bias: torch
 class PagedKV:
     """A paged key/value cache in packed HiF4: for K and for V codes uint8 (pages, kv_heads, page_size,
     head_dim/2) and meta int32 (pages, kv_heads, page_size, head_dim/64).  head_dim 64 or 128, page_size a
-    power of two from 16 to 256.  Holds the tensors, which stay the caller's."""
+    power of two from 16 to 256.  Holds the tensors, which stay the caller's; they cannot be exchanged for others."""
 
     def __init__(self, k_codes: torch.Tensor, k_meta: torch.Tensor, v_codes: torch.Tensor, v_meta: torch.Tensor):
         _cuda(k_codes, "k_codes", (torch.uint8,), 4)
@@ -191,10 +191,13 @@ class PagedKV:
             raise ValueError(f"page_size {p}: a power of two from 16 to 256 wanted")
         if n == 0 or h == 0:
             raise ValueError("the cache has no pages or no heads")
-        self.k_codes, self.k_meta, self.v_codes, self.v_meta = k_codes, k_meta, v_codes, v_meta
-        self.num_pages, self.kv_heads, self.page_size, self.head_dim, self.device = n, h, p, 2 * half, dev
-        self._desc = L.KVCacheDesc(*at, n, p, h, 2 * half)
-        self._ref = ctypes.byref(self._desc)
+        desc = L.KVCacheDesc(*at, n, p, h, 2 * half)
+        self.__dict__.update(k_codes=k_codes, k_meta=k_meta, v_codes=v_codes, v_meta=v_meta, num_pages=n, kv_heads=h,
+                             page_size=p, head_dim=2 * half, device=dev, _desc=desc, _ref=ctypes.byref(desc))
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{name} of a cache is fixed (its tensors' addresses are taken when it is made): "
+                             "make another PagedKV")
 
     @staticmethod
     def empty(num_pages: int, page_size: int, kv_heads: int, head_dim: int, device) -> "PagedKV":

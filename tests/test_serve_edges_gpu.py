@@ -233,3 +233,11 @@ def test_out_beside_an_input_in_one_buffer(T):
             serve.linear(x, meta, codes, out=wide[:, C - 8:C - 8 + N])
 
 
+def test_the_cache_keeps_its_tensors():
+    """A cache describes the tensors it was made with: they and its sizes cannot be replaced."""
+    c = serve.PagedKV.empty(2, 16, 1, 64, "cuda")
+    for name in ("k_codes", "k_meta", "v_codes", "v_meta", "num_pages", "kv_heads", "page_size", "head_dim"):
+        with pytest.raises(AttributeError, match=name):
+            setattr(c, name, getattr(c, name))
+
+
