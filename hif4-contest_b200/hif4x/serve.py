@@ -7,7 +7,8 @@ bf16: a HiF4 value is a bf16 number, so nothing is lost before the fp32 sums
 (fp16 does not reach HiF4's exponents).  Every function launches kernels from
 libhif4x.so on the current stream of the tensors' device, allocates with
 torch and neither synchronises nor reads back, so a call can be captured into
-a CUDA graph.  linalg.check_device_status reports what a kernel found wrong
+a CUDA graph.  There is no backward pass: where gradients are recorded, tensors
+that require one are refused.  linalg.check_device_status reports what a kernel found wrong
 (a page table that names no page of the cache).
 """
 from __future__ import annotations
@@ -36,9 +37,11 @@ def _call(dev: torch.device, name: str, *args) -> None:
 
 
 def _cuda(t: torch.Tensor, name: str, dtypes, dim: int, dev: torch.device | None = None):
-    """The tensor has one of the dtypes and `dim` dimensions and is on `dev` (None: on any GPU)."""
+    """The tensor has one of the dtypes and `dim` dimensions, is on `dev` (None: on any GPU) and waits for no gradient."""
     if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == dim and (
             t.device == dev if dev is not None else t.is_cuda):
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} requires a gradient and this call has none: detach it, or call under torch.no_grad()")
         return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")

@@ -241,3 +241,25 @@ def test_the_cache_keeps_its_tensors():
             setattr(c, name, getattr(c, name))
 
 
+def test_inputs_that_require_a_gradient():
+    """There is no backward pass, so such inputs are refused where gradients are recorded and taken elsewhere."""
+    meta, codes = packed(54, 64, 128)
+    x = torch.randn(2, 128, generator=gen(1), device="cuda").bfloat16()
+    r, bias = torch.zeros(2, 64, device="cuda").bfloat16(), torch.zeros(64, device="cuda")
+    g = lambda t: t.detach().requires_grad_()  # noqa: E731
+    b = Batch([2], [20], 1, 64, 16, 55)
+    kv, q = torch.zeros(2, 1, 64, device="cuda").bfloat16(), torch.zeros(2, 1, 64, device="cuda").bfloat16()
+    calls = [lambda: serve.linear(g(x), meta, codes), lambda: serve.linear(x, meta, codes, bias=g(bias)),
+             lambda: serve.linear(x, meta, codes, residual=g(r)), lambda: serve.linear(x, meta, codes, out=g(r)),
+             lambda: serve.kv_append(b.cache, g(kv), kv, *b.args), lambda: serve.kv_append(b.cache, kv, g(kv), *b.args),
+             lambda: serve.kv_read(b.cache, *b.args, rows=2, out=(g(kv), kv.clone())),
+             lambda: serve.paged_attention(g(q), b.cache, *b.args),
+             lambda: serve.paged_attention(q, b.cache, *b.args, out=g(q))]
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    assert not serve.linear(x, meta, codes).requires_grad
+
+
