@@ -246,7 +246,7 @@ def test_inputs_that_require_a_gradient():
     meta, codes = packed(54, 64, 128)
     x = torch.randn(2, 128, generator=gen(1), device="cuda").bfloat16()
     r, bias = torch.zeros(2, 64, device="cuda").bfloat16(), torch.zeros(64, device="cuda")
-    g = lambda t: t.detach().requires_grad_()  # noqa: E731
+    g = lambda t: t.clone().requires_grad_()  # noqa: E731
     b = Batch([2], [20], 1, 64, 16, 55)
     kv, q = torch.zeros(2, 1, 64, device="cuda").bfloat16(), torch.zeros(2, 1, 64, device="cuda").bfloat16()
     calls = [lambda: serve.linear(g(x), meta, codes), lambda: serve.linear(x, meta, codes, bias=g(bias)),
