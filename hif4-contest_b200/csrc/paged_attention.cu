@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
   uint64_t *vempty = vfull + 2, *sfull = vempty + 2, *pfull = sfull + 4, *odone = pfull + 4;
   uint64_t *drain = odone + 2;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 2);
-  int *found = reinterpret_cast<int *>(tmem_slot + 1);          // sequence, tile
+  int *found = reinterpret_cast<int *>(tmem_slot + 1);          // sequence, tile, first position
   uint8_t *hidden = reinterpret_cast<uint8_t *>(found + 3);     // [4 steps][8 blocks of 16 keys]: 1 without a page
   const CacheArgs &c = a.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -643,6 +643,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
   const int per = (kt.n + a.splits - 1) / a.splits;
   const int first = min(kt.n, split * per), n = min(kt.n, first + per) - first;   // steps of this CTA
 
+  // asked for where a page is none; held in a register through the loops it cost the prologue 0.6 us in spills
+  if (threadIdx.x == 0) found[2] = p_lo;
+
   // ---- Q into shared memory (K-major panels of 64 dims, 128-byte swizzle)
   for (int e = threadIdx.x; e < tiles_here * 128 * (DH / 8); e += THREADS) {
     const int r = e / (DH / 8), q = e % (DH / 8);
@@ -680,17 +683,15 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
     const Loader<DH> ld(c, kh, w, lane);
     Words<DH> cur, next;
     auto key_of = [&](int i) { return kt.key0(first + i, KEYS) + w * 16; };
-    // whether a row of this CTA sees a key of the 16: steps of 128 begin before the window and end behind the sinks,
-    // and pages there may have been given back
-    const int before = a.window ? p_lo - a.window : INT32_MIN;
-    auto seen = [&](int i) {
-      const int k = key_of(i);
-      return i < n && k <= last && (k + 15 > before || k < a.sinks);
-    };
-    auto look = [&](int i) { return seen(i) ? __ldg(pages + (key_of(i) >> c.page_shift)) : -1; };
-    auto check = [&](int i, int page) {   // an id of no page: -1, and reported where a row would have seen the keys
+    auto look = [&](int i) { return i < n && key_of(i) <= last ? __ldg(pages + (key_of(i) >> c.page_shift)) : -1; };
+    // an id of no page: -1, and reported where a row of this CTA would have seen the keys (steps of 128 begin before
+    // the window and end behind the sinks, and pages there may have been given back)
+    auto check = [&](int i, int page) {
       if (page >= 0 && page < c.num_pages) return page;
-      if (lane == 0 && seen(i)) atomicExch(c.status + 1, HIF4X_BAD_PAGE);
+      if (lane == 0 && i < n && key_of(i) <= last) {
+        const int k = key_of(i), p_first = found[2];
+        if (a.window == 0 || k + 15 > p_first - a.window || k < a.sinks) atomicExch(c.status + 1, HIF4X_BAD_PAGE);
+      }
       return -1;
     };
     int now = look(0), nxt = look(1);   // of the step being decoded, of the one after it
