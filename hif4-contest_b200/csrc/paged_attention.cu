@@ -34,6 +34,15 @@
 
 namespace hif4x {
 
+// The partial sums of the keys' shares: n shares of `all` rows (of one query
+// head) each; n == 1: the result goes out directly.
+struct Shares {
+  int n;
+  int64_t all;
+  float *part;   // (n, all, dh)
+  float2 *ml;    // (n, all): reference, weight
+};
+
 struct AttendArgs {
   CacheArgs c;
   const __nv_bfloat16 *q;
@@ -44,9 +53,9 @@ struct AttendArgs {
   float scale;                // times log2(e)
   int window, sinks;          // window 0: all keys
   int most_rows;              // attend_rows_kernel: sequences of up to so many rows; attend_tiles_kernel: of more
-  int splits;
-  float *part;                // (splits, rows, q heads, dh) sums, then (splits, rows, q heads) (reference, weight)
-  float2 *part_ml;
+  Shares sh;
+  int slots;                  // attend_rows_kernel: 0: its sums lie by (token, query head), else by (sequence, key head, row)
+  float2 *mark;               // attend_rows_kernel: the other kernel's first pairs, whose weight -1 says that a row is not its
 };
 
 // Rows (token, query head of a key head) that the call's tensors have of a
@@ -55,6 +64,10 @@ __device__ __forceinline__ int64_t rows_present(const AttendArgs &a, int cu0, in
   if (n_new <= 0 || cu0 < 0 || cu0 >= a.c.rows) return 0;
   return min((int64_t)n_new, a.c.rows - cu0) * a.group;
 }
+
+// Rows of a sequence and key head up to which attend_rows_kernel takes them
+// where both kernels run.
+constexpr int FEW_ROWS = 16;
 
 constexpr int64_t MOST_SPLITS = 64;   // shares of a row's keys (attend_join_kernel: four warps, a lane for each of 16)
 constexpr float kLazy = 8.0f;    // log2 a row's scores may pass its reference by
@@ -231,7 +244,7 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) attend_rows_kernel(const
     }
 
     const KeyTiles tiles(min(max(p_lo, 0), p_hi), p_hi, a.window, a.sinks, 16);
-    const int per = (tiles.n + a.splits - 1) / a.splits;
+    const int per = (tiles.n + a.sh.n - 1) / a.sh.n;
     const int t1 = min(tiles.n, (split + 1) * per);
     int t = split * per + warp;
     // the page of a tile two ahead, the words of the next one
@@ -403,14 +416,16 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) attend_rows_kernel(const
         for (int k = 0; k < 4; k++) v[k] += f * so[w][r][d + k];
       }
       const int head = kh * a.group + (int)(rr % a.group);
-      if (a.splits == 1) {
+      if (a.mark != nullptr && split == 0 && d == 0) a.mark[token * (c.heads * a.group) + head] = make_float2(0.0f, -1.0f);
+      if (a.sh.n == 1) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         *reinterpret_cast<uint2 *>(a.out + token * a.o_row + head * a.o_head + d) =
             make_uint2(pack_bf16(v[0] * inv, v[1] * inv), pack_bf16(v[2] * inv, v[3] * inv));
       } else {
-        const int64_t at = ((int64_t)split * c.rows + token) * (c.heads * a.group) + head;
-        *reinterpret_cast<float4 *>(a.part + at * DH + d) = make_float4(v[0], v[1], v[2], v[3]);
-        if (d == 0) a.part_ml[at] = make_float2(m, l);
+        const int64_t at = split * a.sh.all + (a.slots ? ((int64_t)s * c.heads + kh) * FEW_ROWS + rr
+                                                       : token * (c.heads * a.group) + head);
+        *reinterpret_cast<float4 *>(a.sh.part + at * DH + d) = make_float4(v[0], v[1], v[2], v[3]);
+        if (d == 0) a.sh.ml[at] = make_float2(m, l);
       }
     }
     __syncthreads();
@@ -640,7 +655,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
     p_hi = (int)(room - 1);
   }
   const KeyTiles kt(min(max(p_lo, 0), p_hi), p_hi, a.window, a.sinks, KEYS);
-  const int per = (kt.n + a.splits - 1) / a.splits;
+  const int per = (kt.n + a.sh.n - 1) / a.sh.n;
   const int first = min(kt.n, split * per), n = min(kt.n, first + per) - first;   // steps of this CTA
 
   // asked for where a page is none; held in a register through the loops it cost the prologue 0.6 us in spills
@@ -862,9 +877,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
       const int64_t token = (int64_t)cu0 + rr / a.group;
       const bool mine = rr < r1 && token >= 0 && token < c.rows;
       const int head = kh * a.group + (int)(rr % a.group);
-      const int64_t at = ((int64_t)split * c.rows + token) * (c.heads * a.group) + head;
-      const float inv = a.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
-      if (a.splits > 1 && mine) a.part_ml[at] = make_float2(ref, sum);
+      const int64_t at = split * a.sh.all + token * (c.heads * a.group) + head;
+      const float inv = a.sh.n > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+      if (a.sh.n > 1 && mine) a.sh.ml[at] = make_float2(ref, sum);
 #pragma unroll 1
       for (int c0 = 0; c0 < DH; c0 += 32) {
         uint32_t o[32];
@@ -878,8 +893,8 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
         }
         if (!mine) continue;
         // a chunk of eight dims stands as (0 2 4 6 1 3 5 7)
-        if (a.splits > 1) {
-          float4 *dst = reinterpret_cast<float4 *>(a.part + at * DH + c0);
+        if (a.sh.n > 1) {
+          float4 *dst = reinterpret_cast<float4 *>(a.sh.part + at * DH + c0);
 #pragma unroll
           for (int j = 0; j < 8; j++) {
             const int e = 8 * (j >> 1) + 2 * (j & 1);
@@ -915,40 +930,73 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(const AttendAr
 // The shares of a (row, query head), added in their order: a CTA each, four
 // warps with every fourth share and eight of them on their way at a time (the
 // chain of dependent loads is the time of this kernel), joined in shared
-// memory.
+// memory.  The sums lie by (token, query head); where both kernels ran (BOTH),
+// attend_rows_kernel's are `few`, by (sequence, key head, row).  The grid then
+// is one of the two: few's alone where only its sequences have shares.  In the
+// other one a row of few's is known by its mark, seen when its sums have been
+// read in vain: to ask before would put a load in front of every row's.
+
+// one warp's shares: the sums of its lanes' dims and their (reference, weight)
 template <int DH>
-__global__ void __launch_bounds__(128) attend_join_kernel(const AttendArgs a) {
+__device__ __forceinline__ float2 join_warp(const Shares &sh, int64_t at, int warp, int lane, float (&v)[DH / 32]) {
   constexpr int V = DH / 32;
-  __shared__ float so[4][DH];
-  __shared__ float2 sml[4];
-  const CacheArgs &c = a.c;
-  const int heads = c.heads * a.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t at = blockIdx.x, all = c.rows * heads;
-  const int64_t token = at / heads;
-  const int head = (int)(at - token * heads);
-  if (token < c.cu_new[0] || token >= c.cu_new[c.B]) return;   // rows of no sequence stay as they are
-  // this warp's shares s = warp, warp + 4, ... (at most 16): lane k has the k-th one's reference and weight
+  // shares s = warp, warp + 4, ... (at most 16): lane k has the k-th one's reference and weight
   const int mine = warp + 4 * lane;
-  const float2 ml = mine < a.splits ? a.part_ml[mine * all + at] : make_float2(-INFINITY, 0.0f);
+  const float2 ml = mine < sh.n ? sh.ml[mine * sh.all + at] : make_float2(-INFINITY, 0.0f);
   float m = ml.x;
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
   const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m);   // nothing visible in a share: no part in the sum
-  float l = f * ml.y, v[V];
+  float l = f * ml.y;
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
 #pragma unroll
   for (int k = 0; k < V; k++) v[k] = 0.0f;
 #pragma unroll 8
-  for (int k = 0; k < (a.splits - warp + 3) / 4; k++) {
-    const float *src = a.part + ((warp + 4 * k) * all + at) * DH + lane * V;
+  for (int k = 0; k < (sh.n - warp + 3) / 4; k++) {
+    const float *src = sh.part + ((warp + 4 * k) * sh.all + at) * DH + lane * V;
     const float w = __shfl_sync(0xffffffffu, f, k);
 #pragma unroll
     for (int e = 0; e < V; e++) v[e] += w == 0.0f ? 0.0f : w * src[e];
   }
+  return make_float2(m, l);
+}
+
+template <int DH, bool BOTH>
+__global__ void __launch_bounds__(128, 16) attend_join_kernel(const AttendArgs a, const Shares few, int grid_few) {
+  constexpr int V = DH / 32;
+  __shared__ float so[4][DH];
+  __shared__ float2 sml[4];
+  const CacheArgs &c = a.c;
+  const int heads = c.heads * a.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t at = blockIdx.x;
+  int64_t token;
+  int head;
+  float v[V];
+  float2 ml;
+  if (BOTH && grid_few) {
+    const int r = (int)(at % FEW_ROWS), kh = (int)(at / FEW_ROWS % c.heads), s = (int)(at / FEW_ROWS / c.heads);
+    const int cu0 = c.cu_new[s], n_new = c.cu_new[s + 1] - cu0;
+    if ((int64_t)n_new * a.group > FEW_ROWS || r >= rows_present(a, cu0, n_new)) return;
+    token = (int64_t)cu0 + r / a.group;
+    head = kh * a.group + r % a.group;
+    ml = join_warp<DH>(few, at, warp, lane, v);
+  } else {
+    token = at / heads;
+    head = (int)(at - token * heads);
+    if (token < c.cu_new[0] || token >= c.cu_new[c.B]) return;   // rows of no sequence stay as they are
+    const float mark = BOTH ? a.sh.ml[at].y : 0.0f;
+    ml = join_warp<DH>(a.sh, at, warp, lane, v);
+    if (BOTH && mark < 0.0f) {
+      if (few.n == 1) return;   // its result is there already
+      const int s = find_sequence(c.cu_new, c.B, token, lane & 7, 0xffu << (lane & 24)), kh = head / a.group;
+      ml = join_warp<DH>(few, ((int64_t)s * c.heads + kh) * FEW_ROWS + (token - c.cu_new[s]) * a.group + head - kh * a.group,
+                         warp, lane, v);
+    }
+  }
 #pragma unroll
   for (int e = 0; e < V; e++) so[warp][lane * V + e] = v[e];
-  if (lane == 0) sml[warp] = make_float2(m, l);
+  if (lane == 0) sml[warp] = ml;
   __syncthreads();
   if (threadIdx.x >= DH / 2) return;
   const int d = threadIdx.x * 2;
@@ -973,11 +1021,12 @@ __global__ void __launch_bounds__(128) attend_join_kernel(const AttendArgs a) {
 // of several lengths even out (64 sequences of up to 8192 keys, one tile a turn: 180 us, 289
 // unshared).  No share under 512 keys (eight tiles for each warp; the join is
 // a launch of its own, 4 us), and no more than 2^26 partial sums (256 MB) in
-// all.
-static int attend_splits(int sms, int64_t lanes, int64_t keys, int64_t outputs, bool two) {
+// all.  Beside the tiles kernel (`both`) none under 2048: the join is then
+// launched for sequences that may not be there.
+static int attend_splits(int sms, int64_t lanes, int64_t keys, int64_t outputs, bool two, bool both) {
   const int64_t at_once = (two ? 2 : 3) * (int64_t)sms;
   const int64_t want = lanes * 4 <= at_once * 3 ? at_once / lanes : (12 * (int64_t)sms + lanes - 1) / lanes;
-  const int64_t most = std::max<int64_t>(1, keys / 512);
+  const int64_t most = std::max<int64_t>(1, keys / (both ? 2048 : 512));
   const int64_t room = (int64_t(1) << 26) / std::max<int64_t>(1, outputs);
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, room, MOST_SPLITS}));
 }
@@ -986,15 +1035,17 @@ static int attend_splits(int sms, int64_t lanes, int64_t keys, int64_t outputs, 
 struct AttendPlan {
   bool rows, tiles;          // the kernels that run
   int most_rows;             // rows of a sequence up to which the first one takes it
-  int grid_tiles, splits;
-  int64_t part_floats, work_bytes;
+  int grid_tiles;
+  Shares sh, few;            // of the only kernel, or of the tiles kernel and (n > 0) of the rows kernel beside it
+  int64_t work_bytes;
 };
 
-// Sequences of up to 16 rows (new tokens x query heads of a key head) go to
-// attend_rows_kernel, others to attend_tiles_kernel.  Only the device knows
-// the lengths: where max_new allows for more than 16 rows both kernels run and
-// each passes over the other's sequences, except that a single sequence is the
-// tiles kernel's alone.
+// Sequences of up to FEW_ROWS rows (new tokens x query heads of a key head) go
+// to attend_rows_kernel, others to attend_tiles_kernel.  Only the device knows
+// the lengths: where max_new allows for more rows both kernels run and each
+// passes over the other's sequences, except that a single sequence is the
+// tiles kernel's alone.  Each kernel has its own number of shares: a chunk's
+// tiles fill the GPU by themselves, the long token beside it does not.
 struct AttendSizes {
   int page_size, kv_heads, head_dim, sequences, max_pages, q_heads;
   int64_t rows;
@@ -1008,26 +1059,51 @@ static int attend_plan(const AttendSizes &z, AttendPlan *p) {
   if (sms <= 0) return HIF4X_ERR_LAUNCH;
   const int group = z.q_heads / z.kv_heads;
   const int64_t B = z.sequences, H = z.kv_heads;
-  int64_t keys = (int64_t)z.max_pages * z.page_size;
-  if (z.window > 0) keys = std::min<int64_t>(keys, (int64_t)z.window + z.max_new + z.sinks + 32);
+  // keys that a sequence of up to `fresh` new rows sees at most
+  auto keys_of = [&](int64_t fresh) {
+    const int64_t room = (int64_t)z.max_pages * z.page_size;
+    return z.window > 0 ? std::min<int64_t>(room, z.window + fresh + z.sinks + 32) : room;
+  };
+  const int64_t keys = keys_of(z.max_new);
   p->tiles = (int64_t)z.max_new * group > 16;
   p->rows = !p->tiles || B > 1;
-  p->most_rows = !p->tiles ? INT32_MAX : B > 1 ? 16 : 0;
+  p->most_rows = !p->tiles ? INT32_MAX : B > 1 ? FEW_ROWS : 0;
   p->grid_tiles = 0;
+  const int64_t outs = z.rows * z.q_heads, slots = B * H * FEW_ROWS;
+  p->sh.all = outs;
+  p->few.n = 0;
+  p->few.all = slots;
   if (p->tiles) {
     const int64_t n = z.rows * group / tiles::ROWS + B;
     if (n * H > INT32_MAX) return HIF4X_ERR_UNSUPPORTED;
     p->grid_tiles = (int)n;
     // shares of the keys: as many as fill the SMs once (sequences taken alike), four steps or more to each
     const int64_t busy = B * std::max<int64_t>(1, (z.rows * group + B * tiles::ROWS - 1) / (B * tiles::ROWS)) * H;
-    p->splits = (int)std::max<int64_t>(
-        1, std::min<int64_t>({sms / busy, keys / (4 * tiles::KEYS), (int64_t(1) << 26) / (z.rows * z.q_heads * z.head_dim), MOST_SPLITS}));
+    p->sh.n = (int)std::max<int64_t>(
+        1, std::min<int64_t>({sms / busy, keys / (4 * tiles::KEYS), (int64_t(1) << 26) / (outs * z.head_dim), MOST_SPLITS}));
+    if (p->rows) p->few.n = attend_splits(sms, B * H, keys_of(FEW_ROWS), slots * z.head_dim, true, true);
   } else {
-    p->splits = attend_splits(sms, B * H, keys, z.rows * z.q_heads * z.head_dim, (int64_t)z.max_new * group > 8);
+    p->sh.n = attend_splits(sms, B * H, keys, outs * z.head_dim, (int64_t)z.max_new * group > 8, false);
   }
-  p->part_floats = p->splits > 1 ? (int64_t)p->splits * z.rows * z.q_heads * z.head_dim : 0;
-  p->work_bytes = p->splits > 1 ? p->part_floats * 4 + (int64_t)p->splits * z.rows * z.q_heads * 8 : 0;
+  const int64_t sums = (p->sh.n > 1 ? p->sh.n * outs : 0) + (p->few.n > 1 ? p->few.n * slots : 0);
+  p->work_bytes = sums * (4 * z.head_dim + 8);
   return HIF4X_OK;
+}
+
+// The workspace: all partial sums, then all (reference, weight) pairs.
+static void place_shares(AttendPlan *p, void *work, int head_dim) {
+  float *at = static_cast<float *>(work);
+  for (Shares *s : {&p->sh, &p->few})
+    if (s->n > 1) {
+      s->part = at;
+      at += s->n * s->all * head_dim;
+    }
+  float2 *ml = reinterpret_cast<float2 *>(at);
+  for (Shares *s : {&p->sh, &p->few})
+    if (s->n > 1) {
+      s->ml = ml;
+      ml += s->n * s->all;
+    }
 }
 
 template <int DH>
@@ -1037,7 +1113,7 @@ static int launch_tiles(AttendArgs a, int dev, const AttendPlan &p, cudaStream_t
   // the kernel compares unscaled scores, so its scale is positive: a negative one turns the queries' signs
   const int flip = a.scale < 0.0f;
   a.scale = std::max(std::fabs(a.scale), 1e-35f);
-  const dim3 grid((unsigned)(p.grid_tiles * a.c.heads), (unsigned)p.splits);
+  const dim3 grid((unsigned)(p.grid_tiles * a.c.heads), (unsigned)p.sh.n);
   tiles::attend_tiles_kernel<DH><<<grid, tiles::THREADS, tiles::Cfg<DH>::SMEM, s>>>(a, flip);
   HIF4X_CHECK_LAUNCH();
   return HIF4X_OK;
@@ -1097,9 +1173,8 @@ extern "C" int hif4x_paged_attention(const hif4x_kv_cache *kv, const hif4x_kv_ba
   a.scale = scale * 1.4426950408889634f;
   a.window = window;
   a.sinks = sinks;
-  a.splits = p.splits;
-  a.part = static_cast<float *>(work);
-  a.part_ml = reinterpret_cast<float2 *>(static_cast<float *>(work) + p.part_floats);
+  place_shares(&p, work, kv->head_dim);
+  a.sh = p.sh;
   a.most_rows = p.most_rows;
   cudaStream_t s = (cudaStream_t)stream;
   if (p.tiles) {
@@ -1109,21 +1184,33 @@ extern "C" int hif4x_paged_attention(const hif4x_kv_cache *kv, const hif4x_kv_ba
     if (st != HIF4X_OK) return st;
   }
   if (p.rows) {
-    const dim3 grid((unsigned)batch->sequences, (unsigned)kv->kv_heads, (unsigned)p.splits);
+    AttendArgs r = a;
+    if (p.tiles) {
+      r.sh = p.few;
+      r.slots = 1;
+      r.mark = p.sh.n > 1 ? p.sh.ml : nullptr;
+    }
+    const dim3 grid((unsigned)batch->sequences, (unsigned)kv->kv_heads, (unsigned)r.sh.n);
     const bool two = (int64_t)max_new * a.group > 8;
     if (kv->head_dim == 128) {
-      if (two) attend_rows_kernel<128, 2><<<grid, 128, 0, s>>>(a);
-      else attend_rows_kernel<128, 1><<<grid, 128, 0, s>>>(a);
+      if (two) attend_rows_kernel<128, 2><<<grid, 128, 0, s>>>(r);
+      else attend_rows_kernel<128, 1><<<grid, 128, 0, s>>>(r);
     } else {
-      if (two) attend_rows_kernel<64, 2><<<grid, 128, 0, s>>>(a);
-      else attend_rows_kernel<64, 1><<<grid, 128, 0, s>>>(a);
+      if (two) attend_rows_kernel<64, 2><<<grid, 128, 0, s>>>(r);
+      else attend_rows_kernel<64, 1><<<grid, 128, 0, s>>>(r);
     }
     HIF4X_CHECK_LAUNCH();
   }
-  if (p.splits > 1) {
-    const unsigned blocks = (unsigned)(rows * q_heads);
-    if (kv->head_dim == 128) attend_join_kernel<128><<<blocks, 128, 0, s>>>(a);
-    else attend_join_kernel<64><<<blocks, 128, 0, s>>>(a);
+  if (p.sh.n > 1 || p.few.n > 1) {
+    const int grid_few = p.sh.n == 1;
+    const unsigned blocks = (unsigned)(grid_few ? p.few.all : p.sh.all);
+    if (p.few.n > 0) {
+      if (kv->head_dim == 128) attend_join_kernel<128, true><<<blocks, 128, 0, s>>>(a, p.few, grid_few);
+      else attend_join_kernel<64, true><<<blocks, 128, 0, s>>>(a, p.few, grid_few);
+    } else {
+      if (kv->head_dim == 128) attend_join_kernel<128, false><<<blocks, 128, 0, s>>>(a, p.few, 0);
+      else attend_join_kernel<64, false><<<blocks, 128, 0, s>>>(a, p.few, 0);
+    }
     HIF4X_CHECK_LAUNCH();
   }
   return HIF4X_OK;

@@ -263,3 +263,43 @@ def test_inputs_that_require_a_gradient():
     assert not serve.linear(x, meta, codes).requires_grad
 
 
+# ------------------------------------------------------------------ batches of both kinds
+def work_bytes(page, kvh, dh, B, most, qh, rows, max_new, window=0, sinks=0):
+    need = L.i64()
+    L.call("hif4x_paged_attention_work", page, kvh, dh, B, most, qh, rows, window, sinks, max_new, need)
+    return need.value
+
+
+def test_single_tokens_beside_a_chunk_share_their_keys():
+    """A long token beside a chunk, and a decoding batch whose call does not say max_new: the keys of the single tokens are shared out
+    as they are in a call of their own (the workspace holds a sum for each share, and is bounded)."""
+    slot = 16 * (128 + 2) * 4                                   # sums of a key head's rows of one share, in bytes
+    mixed = work_bytes(64, 8, 128, 2, 1024, 32, 2049, 2048)
+    assert mixed >= 16 * 2 * 8 * slot, mixed
+    unsaid = work_bytes(64, 8, 128, 64, 128, 32, 64, 64)
+    assert unsaid >= 3 * 64 * 8 * slot, unsaid
+    assert max(mixed, unsaid) <= 2 ** 29 + 2 ** 24
+    assert work_bytes(64, 8, 128, 2, 7, 32, 300, 299) == 0      # short contexts: one launch of each kernel
+
+
+@pytest.mark.parametrize("new,lens,qh,kvh,dh,page", [
+    ([1, 200], [20000, 900], 8, 2, 128, 64), ([200, 1], [900, 20000], 8, 2, 128, 64),
+    ([64, 1, 64, 2], [9000, 9000, 300, 7000], 4, 1, 64, 16),     # both kinds in shares
+    ([1] * 9 + [0, 40], [5000 + i for i in range(9)] + [3, 40], 8, 4, 128, 32),
+    ([17, 16, 1, 15], [6000, 6000, 6000, 6000], 1, 1, 64, 16),   # about the border of the two kernels
+    ([5, 6, 5], [6000, 3000, 2], 3, 1, 128, 16)])                # three query heads; rows that see nothing
+@pytest.mark.parametrize("window,sinks", [(0, 0), (2500, 3)])
+def test_batches_of_both_kinds(new, lens, qh, kvh, dh, page, window, sinks):
+    b = Batch(new, lens, kvh, dh, page, 43)
+    q = torch.randn(b.rows + 3, qh, dh, generator=gen(7), device="cuda").bfloat16()
+    first = None
+    for _ in range(5):
+        out = torch.full_like(q, 5.0)
+        serve.paged_attention(q, b.cache, *b.args, window=window, sinks=sinks, out=out)
+        assert (out[b.rows:] == 5).all()                         # padding rows stay as they were
+        first = out if first is None else first
+        assert torch.equal(out, first)
+    linalg.check_device_status()
+    check_attention(b, q, first, window, sinks)
+
+
