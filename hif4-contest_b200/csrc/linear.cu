@@ -362,20 +362,9 @@ extern "C" int hif4x_linear_packed(const void *x, int64_t ldx, const uint32_t *m
   if (!opt_in(linear_kernel, smem_bytes(256), dev) || !a.status) return HIF4X_ERR_LAUNCH;
 
   const int64_t tiles_n = (N + BM - 1) / BM;
-  // x rows of a tile, all tiles alike: of the tilings from the fewest tiles on, the one whose waves of CTAs take
-  // least, a step taking 2.25 cycles a row (shared memory: x in and out) and never under 600 (decoding).
-  // 4096 x 4096 rows: 18 tiles of 240, four waves, instead of 16 of 256, four waves too
-  const int64_t fewest = (T + 255) / 256;
-  int64_t tiles_t = fewest, least = INT64_MAX;
-  for (int64_t n = fewest; n <= fewest + fewest / 4; n++) {
-    const int64_t nt = ((T + n - 1) / n + 15) / 16 * 16;
-    const int64_t cost = ((tiles_n * n + sms - 1) / sms) * std::max<int64_t>(600 * 4, 9 * nt);
-    if (cost < least) {
-      least = cost;
-      tiles_t = n;
-    }
-    if (n - fewest >= 64) break;
-  }
+  // x rows of a tile: as few tiles as hold them, all alike.  A step's decoding takes 600 cycles whatever its rows and
+  // shared memory 2.25 a row (x in and out), 576 at 256: tiles of fewer rows only add steps.
+  int64_t tiles_t = (T + 255) / 256;
   a.nt = (int)(((T + tiles_t - 1) / tiles_t + 15) / 16 * 16);
   tiles_t = (T + a.nt - 1) / a.nt;
   if (tiles_t > 65535) return HIF4X_ERR_UNSUPPORTED;
