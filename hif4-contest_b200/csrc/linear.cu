@@ -369,10 +369,12 @@ extern "C" int hif4x_linear_packed(const void *x, int64_t ldx, const uint32_t *m
   tiles_t = (T + a.nt - 1) / a.nt;
   if (tiles_t > 65535) return HIF4X_ERR_UNSUPPORTED;
   a.nb = (int)(C / 64);
-  // share C out while that gives more SMs a CTA, 4 steps or more to each
+  // share C out while that gives more SMs a CTA; boxes of 4 steps stay whole, so the last CTA may have fewer than the
+  // others, but none has nothing (C = 1088: 8, 8 and 1 steps)
   int ranks = 1;
   while (ranks < MOST_RANKS && tiles_n * tiles_t * ranks * 2 <= sms && a.nb >= 8 * ranks) ranks *= 2;
   a.per = (int)(((a.nb + ranks - 1) / ranks + 3) / 4 * 4);
+  ranks = (a.nb + a.per - 1) / a.per;
   a.T = T;
   a.N = N;
   a.meta = meta;
