@@ -303,3 +303,56 @@ def test_batches_of_both_kinds(new, lens, qh, kvh, dh, page, window, sinks):
     check_attention(b, q, first, window, sinks)
 
 
+# ------------------------------------------------------------------ every scale byte, level bit and code
+def every_byte(shape, seed):
+    """Packed units (shape) x 64 elements with random levels and codes, the scale bytes 0 .. 255 in turn."""
+    g = gen(seed)
+    n = math.prod(shape)
+    meta = torch.randint(-2 ** 23, 2 ** 23, (n,), generator=g, device="cuda") << 8 | torch.arange(n, device="cuda") % 256
+    codes = torch.randint(0, 256, (*shape[:-1], shape[-1] * 32), generator=g, device="cuda", dtype=torch.uint8)
+    return meta.to(torch.int32).view(shape), codes
+
+
+def test_linear_of_every_scale_byte():
+    meta, codes = every_byte((130, 4), 60)
+    x = torch.eye(256, device="cuda").bfloat16()                 # each output is one weight
+    assert torch.equal(serve.linear(x, meta, codes).double(), values64(meta, codes).t())
+
+
+@pytest.mark.parametrize("dh", [64, 128])
+def test_cache_of_every_scale_byte(dh):
+    """kv_read, and V in both attention kernels (a window of one key: the result is that key's V)."""
+    pages, kvh, page = 24, 2, 16
+    shape = (pages, kvh, page, dh // 64)
+    (km, kc), (vm, vc) = every_byte(shape, 61), every_byte(shape, 62)
+    cache = serve.PagedKV(kc, km, vc, vm)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").flip(0)[None].contiguous()
+    n = pages * page
+    order = lambda m, c: values64(m, c)[table[0].long()].transpose(1, 2).reshape(n, kvh, dh)  # noqa: E731
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    k, v = serve.kv_read(cache, i32(0, n), i32(n), table, rows=n)
+    assert torch.equal(k.double(), order(km, kc)) and torch.equal(v.double(), order(vm, vc))
+    q = torch.zeros(n, 4, dh, device="cuda").bfloat16()
+    out = serve.paged_attention(q, cache, i32(0, n), i32(n), table, window=1)
+    assert torch.equal(out.double(), order(vm, vc).repeat_interleave(2, 1))
+    # a row a sequence, each with its own length
+    cu, lens = torch.arange(n + 1, dtype=torch.int32, device="cuda"), torch.arange(1, n + 1, dtype=torch.int32, device="cuda")
+    out = serve.paged_attention(q, cache, cu, lens, table.expand(n, pages).contiguous(), window=1, max_new=1)
+    assert torch.equal(out.double(), order(vm, vc).repeat_interleave(2, 1))
+    linalg.check_device_status()
+
+
+@pytest.mark.parametrize("n", [1, 17])
+@pytest.mark.parametrize("dh", [64, 128])
+def test_attention_with_keys_of_every_scale_byte(n, dh):
+    """K in both attention kernels: sequence s has the scale byte s in all its keys and queries of that much less size."""
+    b = Batch([n] * 256, [n + 9] * 256, 1, dh, 32, 63)
+    E = torch.arange(256, device="cuda") // 4 - 48
+    for s in range(256):
+        ids = b.pages[s, :1].long()
+        b.cache.k_meta[ids] = (b.cache.k_meta[ids] & ~255) | s
+    q = torch.randn(256, n, 1, dh, generator=gen(64), device="cuda") * torch.exp2(-E.float())[:, None, None, None]
+    q = q.reshape(256 * n, 1, dh).bfloat16()
+    check_attention(b, q, serve.paged_attention(q, b.cache, *b.args, max_new=n))
+
+
