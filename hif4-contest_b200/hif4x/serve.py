@@ -114,7 +114,12 @@ def linear(x: torch.Tensor, meta: torch.Tensor, codes: torch.Tensor, bias: torch
     x: (T, C) bf16, unit inner stride, rows a multiple of 8 elements apart, 16-byte aligned.  meta int32
     (N, C/64) and codes uint8 (N, C/2): contiguous.  bias: (N,) fp32 or bf16.  activation: none, relu, gelu
     (by erf), gelu_tanh or silu.  residual: (T, N) bf16, unit inner stride; out: the same, and it may be the
-    residual itself, but lie over no other input.  Sums are fp32 on the tensor cores, rounded once at the end."""
+    residual itself, but lie over no other input.  Sums are fp32 on the tensor cores, rounded once at the end.
+
+    x is taken as it comes.  A weight that linear.calibrate_weight made, or codec.convert with smoothing or
+    rotation, belongs to activations smoothed (times the activation state's s) and, where its mode is 1, rotated:
+    bring x there first, by codec.convert(x, kind=SRC_VALUES, smooth=s, smooth_mode=SMOOTH_MUL, rotate=mode == 1,
+    encode=ENC_NONE, out_x=True), or pass the values that linear.dynamic_activation chose."""
     _cuda(x, "x", (torch.bfloat16,), 2)
     dev = x.device
     _cuda(codes, "codes", (torch.uint8,), 2, dev)

@@ -356,3 +356,70 @@ def test_attention_with_keys_of_every_scale_byte(n, dh):
     check_attention(b, q, serve.paged_attention(q, b.cache, *b.args, max_new=n))
 
 
+# ------------------------------------------------------------------ weights of another space
+def to_weight_space(x, s, mode):
+    """x as the product with a calibrated weight takes it: smoothed and, by mode, rotated."""
+    return codec.convert(x, kind=L.SRC_VALUES, smooth=s, smooth_mode=L.SMOOTH_MUL, rotate=mode == 1,
+                         encode=L.ENC_NONE, out_x=True)["x"].bfloat16()
+
+
+def check_layer(x, w, s, mode, meta, codes):
+    """x brought to the weight's space times the weight is x w^T, up to what the weight's own encode lost."""
+    xt = to_weight_space(x, s, mode)
+    y = serve.linear(xt, meta, codes)
+    check_linear(xt, meta, codes, y)
+    xs, ws = x.float() * s, w / s
+    if mode == 1:
+        xs, ws = codec.rotate64(xs.contiguous()), codec.rotate64(ws.contiguous())
+    wq = values64(meta, codes)
+    want = x.double() @ w.double().t()
+    # the encode's loss; x's rounding to bf16; the fp32 scalings and rotations (sums of 64) of both sides; the result's
+    lost = (xs.double() @ (wq - ws.double()).t()).abs()
+    tol = lost + (2 * BF16 + 200 * 2.0 ** -23) * (xs.double().abs() @ wq.abs().t()) + 200 * 2.0 ** -23 * (
+        xs.double().abs() @ ws.double().abs().t()) + BF16 * want.abs()
+    off = (y.double() - want).abs()
+    assert (off <= tol).all(), f"off by {(off / tol).max().item():.2f} of the tolerance"
+    # and that is little: roundings have a variance of 1/12 of a step's square, a quad's peak is 3.5 steps or more, so
+    # its mean square 3.5^2 / 4: under 3 percent (quads far below their group's peak lose more of less)
+    assert (y.double() - want).square().mean() < 0.05 * want.square().mean()
+
+
+@pytest.mark.parametrize("mode", [0, 1])
+def test_product_in_a_smoothed_and_rotated_space(mode):
+    T, N, C = 33, 200, 512
+    x = torch.randn(T, C, generator=gen(70), device="cuda").bfloat16()
+    x[:, ::50] *= 16
+    w = torch.randn(N, C, generator=gen(71), device="cuda")
+    s = x.float().abs().amax(0).clamp_min(0.1).rsqrt()
+    p = codec.convert(w, kind=L.SRC_VALUES, smooth=s, smooth_mode=L.SMOOTH_DIV, rotate=mode == 1, dict5=False, packed=True)
+    check_layer(x, w, s, mode, p["meta"], p["codes"])
+
+
+@pytest.mark.parametrize("name", ["lin_c1024", "lin_c2560"])
+def test_product_with_a_calibrated_weight(name, tmp_path):
+    """calibrate_weight's result, and the same from the file that a conversion leaves."""
+    import sys
+
+    from conftest import GOLDEN
+    if GOLDEN not in sys.path:
+        sys.path.insert(0, GOLDEN)
+    import pipeline_cases as pc
+
+    from hif4x import linear, shard, weightset
+    wpair, calib, tests, _ = pc.linear_inputs(name)
+    dev = torch.device("cuda", torch.cuda.current_device())
+    cuda = lambda pair: [t.cuda() for t in pair]  # noqa: E731
+    path = weightset.convert_to_dir([(name, cuda(wpair), [cuda(c) for c in calib], cuda(tests[0]))], str(tmp_path))[name]
+    rec = torch.load(path, weights_only=False)
+    res = linear.calibrate_weight(wpair[0], wpair[1], calib)
+    x, w = linear.decode_pair(tests[0], dev).bfloat16(), linear.decode_pair(wpair, dev)
+    for packed_, st in ((rec["packed"].cuda(), rec["activation_state"]),
+                        (shard.pack_params(res["weight_params"]), res["activation_state"])):
+        meta, codes = shard.unpack_params(packed_, rec["rows"], rec["cols"])
+        check_layer(x, w, st["s"].float().to(dev), st["mode"], meta, codes)
+        # activations converted too: their values are bf16 numbers of the same space
+        p = linear.dynamic_activation(*tests[0], st, return_device=True)
+        xq = codec.decode(p, torch.bfloat16)
+        check_linear(xq, meta, codes, serve.linear(xq, meta, codes))
+
+
