@@ -990,8 +990,9 @@ __global__ void __launch_bounds__(128, 16) attend_join_kernel(const AttendArgs a
     if (BOTH && mark < 0.0f) {
       if (few.n == 1) return;   // its result is there already
       const int s = find_sequence(c.cu_new, c.B, token, lane & 7, 0xffu << (lane & 24)), kh = head / a.group;
-      ml = join_warp<DH>(few, ((int64_t)s * c.heads + kh) * FEW_ROWS + (token - c.cu_new[s]) * a.group + head - kh * a.group,
-                         warp, lane, v);
+      const int64_t r = (token - c.cu_new[s]) * a.group + head - kh * a.group;
+      if (s >= c.B || r < 0 || r >= FEW_ROWS) return;   // a cu_new that falls: no such sums
+      ml = join_warp<DH>(few, ((int64_t)s * c.heads + kh) * FEW_ROWS + r, warp, lane, v);
     }
   }
 #pragma unroll

@@ -423,3 +423,16 @@ def test_product_with_a_calibrated_weight(name, tmp_path):
         check_linear(xq, meta, codes, serve.linear(xq, meta, codes))
 
 
+def test_a_description_that_falls_reads_nothing_else():
+    """cu_new must not fall; where it does all the same, the rows concerned are undefined, no place outside the call's
+    tensors is touched, and the next call is right."""
+    b = Batch([12, 12, 40], [9000, 9000, 9000], 1, 64, 16, 58)
+    q = torch.randn(b.rows, 1, 64, generator=gen(59), device="cuda").bfloat16()
+    bad = torch.tensor([0, 12, 4, 64], dtype=torch.int32, device="cuda")
+    serve.paged_attention(q, b.cache, bad, b.len, b.pages)
+    torch.cuda.synchronize()
+    linalg.check_device_status()
+    check_attention(b, q, serve.paged_attention(q, b.cache, *b.args))
+    linalg.check_device_status()
+
+
