@@ -17,9 +17,10 @@
 //            32 columns of bf16 pairs to tensor memory, where the MMA reads A
 //            from.  (A decoding warp alone issues an instruction in 5 to 6
 //            cycles: with two warps a scheduler a step took 830 cycles, with
-//            four 600, of which the ALU pipe is busy for 350.)  W's tile never passes shared memory as bf16: that leaves
-//            shared memory's bandwidth to x alone (a 128 x 256 x 64 step would
-//            otherwise write and read 96 KB there, more than its MMA time).
+//            four 600, of which the ALU pipe is busy for 350.)  W's tile never
+//            passes shared memory as bf16: that leaves shared memory's
+//            bandwidth to x alone (a 128 x 256 x 64 step would otherwise write
+//            and read 96 KB there, more than its MMA time).
 // C is shared out over a cluster of up to 4 CTAs where the tiles alone do not
 // fill the GPU; the partial sums meet through distributed shared memory and
 // are added in rank order, so results do not depend on timing.

@@ -333,7 +333,10 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) attend_rows_kernel(const
               }
             }
         }
-        // ---- weights, transposed for the second product
+        // ---- weights, transposed for the second product.  They go to bf16 there, which is off by half a step (2^-8 of
+        // a weight at most) from key to key alike: about the size of the result's own rounding (against 64 bits 0.0022
+        // of the result where the rounding alone gives 0.0016).  A low part beside it would be a second product over
+        // V, whose decoded pairs are in registers for one.  The weights' sum stays fp32.
         uint32_t pb[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -540,7 +543,10 @@ struct Loader {
   }
 };
 
-// weights of 32 columns: p = 2^(s scale - ref), summed (pairs of sums) and packed
+// weights of 32 columns: p = 2^(s scale - ref), summed in fp32 (pairs of sums)
+// and packed to bf16 for the second product, as in attend_rows_kernel; a low
+// part would need columns of tensor memory that are not there, and half as
+// much tensor-core work again.
 __device__ __forceinline__ void weights32(const uint32_t (&s)[32], u64 scale2, u64 nref2, u64 &sum2, uint32_t *p) {
 #pragma unroll
   for (int j = 0; j < 16; j++) {
@@ -1017,10 +1023,10 @@ __global__ void __launch_bounds__(128, 16) attend_join_kernel(const AttendArgs a
 
 // Shares of the keys of one (sequence, key head) in attend_rows_kernel.  Few
 // lanes (sequence, key head): as many shares as the SMs hold CTAs at once (a
-// second wave would leave most of them idle; 65536 keys of one sequence: 50
-// us, 91 with three waves).  Many: twelve CTAs for every SM, so that sequences
-// of several lengths even out (64 sequences of up to 8192 keys, one tile a turn: 180 us, 289
-// unshared).  No share under 512 keys (eight tiles for each warp; the join is
+// second wave would leave most of them idle; 65536 keys of one sequence: 46 us
+// in 55 shares, 61 in 27, 56 in 64).  Many: twelve CTAs for every SM, so that
+// sequences of several lengths even out (64 sequences of up to 8192 keys: 168
+// us in the four shares this gives, 217 unshared, 205 in twelve).  No share under 512 keys (eight tiles for each warp; the join is
 // a launch of its own, 4 us), and no more than 2^26 partial sums (256 MB) in
 // all.  Beside the tiles kernel (`both`) none under 2048: the join is then
 // launched for sequences that may not be there.
