@@ -203,9 +203,14 @@ class PagedKV:
         self.__dict__.update(k_codes=k_codes, k_meta=k_meta, v_codes=v_codes, v_meta=v_meta, num_pages=n, kv_heads=h,
                              page_size=p, head_dim=2 * half, device=dev, _desc=desc, _ref=ctypes.byref(desc))
 
+    _FIXED = frozenset(("k_codes", "k_meta", "v_codes", "v_meta", "num_pages", "kv_heads", "page_size", "head_dim",
+                        "device", "_desc", "_ref"))
+
     def __setattr__(self, name, value):
-        raise AttributeError(f"{name} of a cache is fixed (its tensors' addresses are taken when it is made): "
-                             "make another PagedKV")
+        if name in self._FIXED:
+            raise AttributeError(f"{name} of a cache is fixed (its tensors' addresses are taken when it is made): "
+                                 "make another PagedKV")
+        object.__setattr__(self, name, value)
 
     @staticmethod
     def empty(num_pages: int, page_size: int, kv_heads: int, head_dim: int, device) -> "PagedKV":

@@ -436,3 +436,9 @@ def test_a_description_that_falls_reads_nothing_else():
     linalg.check_device_status()
 
 
+def test_a_cache_takes_other_attributes():
+    c = serve.PagedKV.empty(2, 16, 1, 64, "cuda")
+    c.layer = 3
+    assert c.layer == 3
+
+
