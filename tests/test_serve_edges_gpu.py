@@ -442,3 +442,32 @@ def test_a_cache_takes_other_attributes():
     assert c.layer == 3
 
 
+def test_a_graph_of_both_kinds_with_other_lengths():
+    """One captured call, replayed with descriptions that make every sequence single tokens, chunks or nothing in
+    turn: each replay is right, and equal to an eager call of the same sizes."""
+    kvh, dh, page, rows, qh = 2, 128, 32, 90, 8
+    cases = [([1, 80, 2, 7], [9000, 4000, 5000, 9000]), ([80, 1, 9, 0], [9000, 30, 9000, 7000]),
+             ([0, 0, 90, 0], [1, 1, 6000, 1]), ([4, 4, 4, 4], [9000, 8000, 7000, 3]), ([1, 1, 1, 1], [9000, 2, 5000, 4097])]
+    b = Batch([20] * 4, [9000] * 4, kvh, dh, page, 57)
+    q = torch.randn(rows, qh, dh, generator=gen(58), device="cuda").bfloat16()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        serve.paged_attention(q, b.cache, *b.args)
+    torch.cuda.current_stream().wait_stream(side)
+    out = torch.empty_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        serve.paged_attention(q, b.cache, *b.args, out=out)
+    for new, lens in cases + cases[::-1]:
+        b.new, b.lens, b.rows = new, lens, sum(new)
+        b.cu.copy_(torch.tensor(np.concatenate([[0], np.cumsum(new)]), dtype=torch.int32))
+        b.len.copy_(torch.tensor(lens, dtype=torch.int32))
+        out.fill_(5.0)
+        graph.replay()
+        assert (out[b.rows:] == 5).all()
+        check_attention(b, q, out)
+        assert torch.equal(out[:b.rows], serve.paged_attention(q, b.cache, *b.args)[:b.rows])
+    linalg.check_device_status()
+
+
