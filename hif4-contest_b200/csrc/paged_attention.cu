@@ -1026,10 +1026,11 @@ __global__ void __launch_bounds__(128, 16) attend_join_kernel(const AttendArgs a
 // second wave would leave most of them idle; 65536 keys of one sequence: 46 us
 // in 55 shares, 61 in 27, 56 in 64).  Many: twelve CTAs for every SM, so that
 // sequences of several lengths even out (64 sequences of up to 8192 keys: 168
-// us in the four shares this gives, 217 unshared, 205 in twelve).  No share under 512 keys (eight tiles for each warp; the join is
-// a launch of its own, 4 us), and no more than 2^26 partial sums (256 MB) in
-// all.  Beside the tiles kernel (`both`) none under 2048: the join is then
-// launched for sequences that may not be there.
+// us in the four shares this gives, 217 unshared, 205 in twelve).  No share
+// under 512 keys (eight tiles for each warp; the join is a launch of its own,
+// 4 us), and no more than 2^26 partial sums (256 MB) in all.  Beside the tiles
+// kernel (`both`) none under 2048: the join is then launched for sequences
+// that may not be there.
 static int attend_splits(int sms, int64_t lanes, int64_t keys, int64_t outputs, bool two, bool both) {
   const int64_t at_once = (two ? 2 : 3) * (int64_t)sms;
   const int64_t want = lanes * 4 <= at_once * 3 ? at_once / lanes : (12 * (int64_t)sms + lanes - 1) / lanes;
